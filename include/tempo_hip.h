@@ -743,6 +743,154 @@ int tmp_arrow_import(const struct ArrowArray *array, const struct ArrowSchema *s
                      size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Attention over ordered series (no counterpart in the reference, whose windows have fixed weights:
+ * python/tempo/tsdf.py:615-635 EMA, :637-671 withLookbackFeatures).  Rows are in (key, ts) order, one
+ * series after the other, as tmp_sort_order leaves them; offsets is a DEVICE array of n_series + 1
+ * ascending row numbers, series s being rows [offsets[s], offsets[s + 1]).  Rows before the first or
+ * behind the last offset belong to no series: their results are zeros and nothing reads them.  NULL
+ * offsets: one series of all rows.
+ *
+ * Row arrays: element d of head h of row r at p[r * row_stride + h * head_stride + d] (strides in
+ * elements), of type TMP_BF16 or TMP_F32.  Sums, softmax statistics and states are 32-bit floats.
+ * A value that is not finite makes the results that depend on it not finite (NaN or infinite), and
+ * no other ones.  Calls enqueue work and return; none of them waits for the device.
+ */
+#define TMP_BF16 0
+#define TMP_F32 1
+#define TMP_MAX_HEAD_DIM 128
+#define TMP_MAX_SINKS 32
+
+typedef struct {
+  void *p;
+  int64_t row_stride;
+  int64_t head_stride;
+} tmp_rows;
+
+/* ---------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head: S_i = exp(log_decay[h]) S_{i-1} + k_i v_i^T,
+ * out_i = scale S_i^T q_i; S before a series' first row is state_in[series] (NULL: zero), behind its
+ * last row state_out[series] (NULL: not wanted).  States are [n_series][heads][dim_k][dim_v] float;
+ * log_decay[heads] float, <= 0 (-infinity: only the row itself).  scale > 0.
+ *
+ * _grad: dq, dk, dv from dout and, when dstate_out is given, the gradient of state_out; dstate_in
+ * (NULL: not wanted) receives the gradient of state_in.  log_decay has no gradient.  out / state_out
+ * are not read.  The workspace is the same for both.
+ */
+typedef struct {
+  int64_t n;
+  int32_t n_series;
+  const int64_t *offsets;
+  int32_t type;
+  int32_t heads;
+  int32_t dim_k, dim_v;
+  float scale;
+  const float *log_decay;
+  tmp_rows q, k, v, out;
+  const float *state_in;
+  float *state_out;
+  tmp_rows dout, dq, dk, dv;
+  const float *dstate_out;
+  float *dstate_in;
+} tmp_decay_attention_args;
+
+size_t tmp_decay_attention_workspace_bytes(const tmp_decay_attention_args *a);
+int tmp_decay_attention(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream);
+int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Softmax attention over a sliding window: row i of a series sees its rows j <= i with j > i - window
+ * and the series' first `sinks` (<= TMP_MAX_SINKS) rows.  heads is a multiple of kv_heads; query head h
+ * reads key/value head h / (heads / kv_heads).  lse[n][heads] (NULL: not wanted; -infinity for rows of
+ * no series) is log sum exp of the scaled scores, which _grad needs beside out.  scale > 0.
+ */
+typedef struct {
+  int64_t n;
+  int32_t n_series;
+  const int64_t *offsets;
+  int32_t type;
+  int32_t heads, kv_heads;
+  int32_t dim_k, dim_v;
+  int64_t window;
+  int32_t sinks;
+  float scale;
+  tmp_rows q, k, v, out;
+  float *lse;
+  tmp_rows dout, dq, dk, dv;
+} tmp_window_attention_args;
+
+int tmp_window_attention(const tmp_window_attention_args *a, void *stream);
+size_t tmp_window_attention_grad_workspace_bytes(const tmp_window_attention_args *a);
+int tmp_window_attention_grad(const tmp_window_attention_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Single rows.  A slot holds what one series' rows so far leave: for the decay form its state
+ * [heads][dim_k][dim_v] (float), for the window form a cache of window + sinks rows and length[slot], the
+ * rows seen so far.  Row t of a series lies at place t (t < sinks) or sinks + (t - sinks) % window.
+ * Row b of the call is the next row of slot slots[b] (NULL: slot b): it is added first, then read with the
+ * others, and the slot is changed in place.  A row whose slot is outside [0, n_slots) or is named by an
+ * earlier row of the same call changes nothing and results in NaN.
+ *
+ * tmp_window_cache_write fills slots from whole series (the rows that tmp_window_attention was called
+ * on): slot slots[s] (NULL: s) afterwards holds series s and nothing else.  A series whose slot is out of
+ * range or named by an earlier series is left out.
+ */
+typedef struct {
+  int64_t n;
+  int32_t n_slots;
+  const int32_t *slots;
+  int32_t type;
+  int32_t heads;
+  int32_t dim_k, dim_v;
+  float scale;
+  const float *log_decay;
+  tmp_rows q, k, v, out;
+  float *state;
+} tmp_decay_attention_step_args;
+
+int tmp_decay_attention_step(const tmp_decay_attention_step_args *a, void *stream);
+
+typedef struct {
+  void *p;
+  int64_t slot_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+} tmp_cache;
+
+typedef struct {
+  int64_t n;
+  int32_t n_slots;
+  const int32_t *slots;
+  int32_t type;
+  int32_t heads, kv_heads;
+  int32_t dim_k, dim_v;
+  int32_t window, sinks;
+  float scale;
+  tmp_rows q, k, v, out;
+  tmp_cache k_cache, v_cache;
+  int64_t *length;
+} tmp_window_attention_step_args;
+
+size_t tmp_window_attention_step_workspace_bytes(const tmp_window_attention_step_args *a);
+int tmp_window_attention_step(const tmp_window_attention_step_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
+typedef struct {
+  int64_t n;
+  int32_t n_series;
+  const int64_t *offsets;
+  int32_t n_slots;
+  const int32_t *slots;
+  int32_t type;
+  int32_t kv_heads;
+  int32_t dim_k, dim_v;
+  int32_t window, sinks;
+  tmp_rows k, v;
+  tmp_cache k_cache, v_cache;
+  int64_t *length;
+} tmp_window_cache_write_args;
+
+int tmp_window_cache_write(const tmp_window_cache_write_args *a, void *stream);
+
+/* ---------------------------------------------------------------------------------------
  * Diagnostics: per-kernel device time (no counterpart in the reference; Spark exposes stage
  * timings through its UI).  While enabled, every kernel launch of the entry points above is
  * bracketed by two HIP events on its launch stream.  tmp_profile_enable(1) creates the event

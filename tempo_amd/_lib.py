@@ -166,6 +166,52 @@ ARROW_I32, ARROW_I64, ARROW_F64, ARROW_I64_RAW = 0, 1, 2, 3
 
 # every symbol include/tempo_hip.h declares: name -> (restype, argtypes)
 _OP = lambda argt: (C.c_int, [C.POINTER(argt), _vp, C.c_size_t, _vp])
+class RowsRef(C.Structure):
+    _fields_ = [("p", _vp), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class CacheRef(C.Structure):
+    _fields_ = [("p", _vp), ("slot_stride", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class DecayAttentionArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("n_series", C.c_int32), ("offsets", _vp), ("type", C.c_int32),
+                ("heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32), ("scale", C.c_float),
+                ("log_decay", _vp), ("q", RowsRef), ("k", RowsRef), ("v", RowsRef), ("out", RowsRef),
+                ("state_in", _vp), ("state_out", _vp), ("dout", RowsRef), ("dq", RowsRef), ("dk", RowsRef),
+                ("dv", RowsRef), ("dstate_out", _vp), ("dstate_in", _vp)]
+
+
+class WindowAttentionArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("n_series", C.c_int32), ("offsets", _vp), ("type", C.c_int32),
+                ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32),
+                ("window", C.c_int64), ("sinks", C.c_int32), ("scale", C.c_float), ("q", RowsRef),
+                ("k", RowsRef), ("v", RowsRef), ("out", RowsRef), ("lse", _vp), ("dout", RowsRef),
+                ("dq", RowsRef), ("dk", RowsRef), ("dv", RowsRef)]
+
+
+class DecayAttentionStepArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("n_slots", C.c_int32), ("slots", _vp), ("type", C.c_int32),
+                ("heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32), ("scale", C.c_float),
+                ("log_decay", _vp), ("q", RowsRef), ("k", RowsRef), ("v", RowsRef), ("out", RowsRef),
+                ("state", _vp)]
+
+
+class WindowAttentionStepArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("n_slots", C.c_int32), ("slots", _vp), ("type", C.c_int32),
+                ("heads", C.c_int32), ("kv_heads", C.c_int32), ("dim_k", C.c_int32), ("dim_v", C.c_int32),
+                ("window", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float), ("q", RowsRef),
+                ("k", RowsRef), ("v", RowsRef), ("out", RowsRef), ("k_cache", CacheRef),
+                ("v_cache", CacheRef), ("length", _vp)]
+
+
+class WindowCacheWriteArgs(C.Structure):
+    _fields_ = [("n", C.c_int64), ("n_series", C.c_int32), ("offsets", _vp), ("n_slots", C.c_int32),
+                ("slots", _vp), ("type", C.c_int32), ("kv_heads", C.c_int32), ("dim_k", C.c_int32),
+                ("dim_v", C.c_int32), ("window", C.c_int32), ("sinks", C.c_int32), ("k", RowsRef),
+                ("v", RowsRef), ("k_cache", CacheRef), ("v_cache", CacheRef), ("length", _vp)]
+
+
 _WS = lambda argt: (C.c_size_t, [C.POINTER(argt)])
 SYMBOLS = {
     "tmp_abi_version": (C.c_int, []),
@@ -206,6 +252,16 @@ SYMBOLS = {
     "tmp_arrow_import_workspace_bytes": (C.c_size_t, [C.POINTER(ArrowArray), C.POINTER(ArrowSchema)]),
     "tmp_arrow_import": (C.c_int, [C.POINTER(ArrowArray), C.POINTER(ArrowSchema), C.c_int32, _vp, _vp,
                                    C.POINTER(C.c_int64), _vp, C.c_size_t, _vp]),
+    "tmp_decay_attention_workspace_bytes": _WS(DecayAttentionArgs),
+    "tmp_decay_attention": _OP(DecayAttentionArgs),
+    "tmp_decay_attention_grad": _OP(DecayAttentionArgs),
+    "tmp_decay_attention_step": (C.c_int, [C.POINTER(DecayAttentionStepArgs), _vp]),
+    "tmp_window_attention": (C.c_int, [C.POINTER(WindowAttentionArgs), _vp]),
+    "tmp_window_attention_grad_workspace_bytes": _WS(WindowAttentionArgs),
+    "tmp_window_attention_grad": _OP(WindowAttentionArgs),
+    "tmp_window_attention_step_workspace_bytes": _WS(WindowAttentionStepArgs),
+    "tmp_window_attention_step": _OP(WindowAttentionStepArgs),
+    "tmp_window_cache_write": (C.c_int, [C.POINTER(WindowCacheWriteArgs), _vp]),
     "tmp_profile_enable": (C.c_int, [C.c_int]),
     "tmp_profile_reset": (C.c_int, []),
     "tmp_profile_count": (C.c_int, []),

@@ -1,0 +1,491 @@
+// Linear attention with a decay for each head over the rows of each series:
+//
+//   S_i = lambda S_{i-1} + k_i v_i^T      o_i = scale S_i^T q_i      lambda = exp(log_decay[head])
+//
+// The state is an exponential moving average of the outer products k v^T.  Rows are worked on in pieces
+// of up to 64 of one series, with r the row's place in the piece and X the state before it:
+//
+//   o_r = scale (lambda^{r+1} X^T q_r + sum_{s<=r} lambda^{r-s} (q_r.k_s) v_s)
+//   X  <- lambda^len X + sum_s lambda^{len-1-s} k_s v_s^T
+//
+// Backward (G_i = scale q_i do_i^T + lambda G_{i+1}, the same recurrence from the last row to the first):
+//   dq_i = scale S_i do_i     dk_i = G_i v_i     dv_i = G_i^T k_i     dS_0 = lambda G_1
+// are three walks of the same kernel with the roles of the rows exchanged; the walks towards the first
+// row keep Y = lambda G, so that o takes lambda^r of it and the update lambda^{len-s}.
+//
+// The table is cut into sections of rows that are walked side by side.  Where a series reaches over a
+// section's start, a first launch walks each section for the state it adds (keys and values only) and a
+// second one strings these together (an elementwise scan over the sections); sections that end with a
+// series' end, as with sequences of equal length, are skipped by both.
+#include <string.h>
+
+#include "series_tile.h"
+
+namespace tmp {
+
+constexpr int DA_PIECE = 64;
+
+struct DecayParams {
+  Series s;
+  Rows q, k, v, out;
+  const float *log_decay;
+  const float *state_in;  // [n_series][heads][dk][dv]
+  float *state_out;
+  float *carry;  // [sections][heads][dk][dv]: the state before a section's first row
+  int32_t *link;  // [sections]: how carry comes about, see decay_scan_kernel
+  int32_t heads, section, sections;
+  int32_t reverse, transposed;  // walk from the last row; states lie as [dv][dk] of this walk's roles
+  float scale, in_by, out_by;   // of rows, and of states read and written
+};
+
+// lambda^m with m >= 0; lambda may be 0 (log2 = -infinity).
+__device__ inline float power(float log2_decay, int m) { return m == 0 ? 1.f : exp2_hw(log2_decay * (float)m); }
+
+// The series that the row at walk position `pos` lies in, in walk positions.  index -1: a stretch of rows
+// that belong to none.
+__device__ inline Span walk_span(const DecayParams &p, int pos) {
+  const int n = p.s.n, row = p.reverse ? n - 1 - pos : pos;
+  const int c = count_le(p.s, row, 0, p.s.n_series + 1);
+  Span sp = span_at(p.s, c, row);
+  if (sp.start > row) {
+    sp.index = -1;
+    int64_t end = n;
+    if (!p.reverse && c < 1) end = p.s.offsets[0];
+    if (p.reverse && c > p.s.n_series) end = n - p.s.offsets[p.s.n_series];
+    sp.start = pos;
+    sp.end = end > n ? n : end <= pos ? pos + 1 : (int)end;
+    return sp;
+  }
+  if (p.reverse) {
+    const int a = n - sp.end;
+    sp.end = n - sp.start;
+    sp.start = a;
+  }
+  return sp;
+}
+
+// A wave's state: all of dk, 32 of dv.  Tile t's register x is dk = 32 t + 16 (x / 8) + 8 (lane / 32) + x % 8,
+// the lane is dv = strip + pi(lane % 32).
+template <int NT> __device__ inline void state_load(f32x16 (&st)[NT], const float *p, int kd, int vd, bool transposed, float by) {
+  const int h8 = (lane_id() >> 5) * 8, dv = (threadIdx.x >> 6) * 32 + pi_of(lane_id() & 31);
+  asm volatile("" : "+v"(vd), "+v"(kd));  // (keeps the addresses from being held in registers over the walk)
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int dk = 32 * t + 16 * (x >> 3) + h8 + (x & 7);
+      st[t][x] = dk < kd && dv < vd ? p[transposed ? dv * kd + dk : dk * vd + dv] * by : 0.f;
+    }
+}
+template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], float *p, int kd, int vd, bool transposed, float by) {
+  const int h8 = (lane_id() >> 5) * 8, dv = (threadIdx.x >> 6) * 32 + pi_of(lane_id() & 31);
+  asm volatile("" : "+v"(vd), "+v"(kd));  // (keeps the addresses from being held in registers over the walk)
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int dk = 32 * t + 16 * (x >> 3) + h8 + (x & 7);
+      if (dk < kd && dv < vd) p[transposed ? dv * kd + dk : dk * vd + dv] = st[t][x] * by;
+    }
+}
+
+// X <- lambda^len X + K^T diag(lambda^{len-1-s+post}) V.  The weighted values do not fit bfloat16; they
+// enter as the sum of two such numbers (2^-18 of a term), three where the state itself is returned (2^-27).
+template <int D> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int b, const float *w, bf16x8 v, bool exact) {
+  bf16x8 hi, lo, rest;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = (float)v[e] * w[e];
+    hi[e] = (__bf16)x;
+    const float y = x - (float)hi[e];
+    lo[e] = (__bf16)y;
+    rest[e] = (__bf16)(y - (float)lo[e]);
+  }
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) {
+    const bf16x8 kf = col_frag<D>(kt, 16 * b, 32 * t);
+    st[t] = mma(kf, hi, st[t]);
+    st[t] = mma(kf, lo, st[t]);
+    if (exact) st[t] = mma(kf, rest, st[t]);
+  }
+}
+template <int D> __device__ inline void state_add(f32x16 (&st)[D / 32], const float *kt, int b, const float *w, f32x8 v, bool) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= w[e];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, 16 * b, 32 * t), v, st[t]);
+}
+
+// OUT: walks a section and writes its rows.  Otherwise: walks the rows of the section that belong to the
+// series which goes on behind it, and leaves the state that they make in carry[section + 1].
+template <typename T, int D, bool OUT>
+__global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
+  constexpr int NT = D / 32, THREADS = D * 2;
+  const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
+  const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = (threadIdx.x >> 6) * 32;
+  const int kd = p.k.dim, vd = p.v.dim;
+  const int64_t per_state = (int64_t)kd * vd;
+  const int sec0 = sec * p.section, sec1 = sec0 + p.section < p.s.n ? sec0 + p.section : p.s.n;
+  int pos = sec0;
+  Span sp;
+  if (!OUT) {
+    sp = walk_span(p, sec1 - 1);
+    const bool on = sp.index >= 0 && sp.end > sec1;
+    if (head == 0 && threadIdx.x == 0) p.link[sec + 1] = !on ? 0 : sp.start < sec0 ? 2 : 1;
+    if (!on) return;
+    pos = sp.start > sec0 ? sp.start : sec0;
+  } else {
+    sp = walk_span(p, sec0);
+  }
+  extern __shared__ __align__(16) unsigned char smem[];
+  T *kt = (T *)smem, *vt = kt + DA_PIECE * D, *qt = vt + DA_PIECE * D;
+  __shared__ int flag[2];
+  if (threadIdx.x < 2) flag[threadIdx.x] = 0;
+  const float ld = p.log_decay[head] * kLog2e;
+  const int post = p.reverse ? 1 : 0;
+  const T *qp = head_of<T>(p.q, head), *kp = head_of<T>(p.k, head), *vp = head_of<T>(p.v, head);
+  float wd[16], wo[16];  // lambda^{i-j} of a 32 x 32 piece on the diagonal, and of the one below it
+  if (OUT)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int j = 16 * (x >> 3) + h8 + (x & 7);
+      wd[x] = j <= l31 ? power(ld, l31 - j) : 0.f;
+      wo[x] = power(ld, 32 + l31 - j);
+    }
+  const float into[2] = {power(ld, l31 + 1 - post), power(ld, l31 + 33 - post)};
+  f32x16 st[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) st[t] = zero16();
+  bool has = false, fresh = true;
+  Staged<T, D, DA_PIECE, THREADS> qs, ks, vs;
+  auto fetch = [&](int at, int len) {
+    const int64_t first = p.reverse ? (int64_t)p.s.n - 1 - at : at;
+    const int step = p.reverse ? -1 : 1;
+    ks.load(kp, p.k.row, kd, p.k.vec, first, step, len);
+    vs.load(vp, p.v.row, vd, p.v.vec, first, step, len);
+    if (OUT) qs.load(qp, p.q.row, p.q.dim, p.q.vec, first, step, len);
+  };
+  auto length = [&](int at, const Span &s) {
+    int e = s.end < sec1 ? s.end : sec1;
+    return e - at < DA_PIECE ? e - at : DA_PIECE;
+  };
+  int len = length(pos, sp), turn = 0;
+  fetch(pos, sp.index < 0 ? 0 : len);
+  while (true) {
+    __syncthreads();
+    ks.store(kt);
+    if (vs.store(vt)) flag[turn] = 1;
+    if (OUT) qs.store(qt);
+    if (threadIdx.x == 0) flag[turn ^ 1] = 0;
+    __syncthreads();
+    const bool dirty = OUT && flag[turn];
+    turn ^= 1;
+    const int next = pos + len;
+    Span nsp = sp;
+    int nlen = 0;
+    if (next < sec1) {
+      if (next >= sp.end) nsp = walk_span(p, next);
+      nlen = length(next, nsp);
+      fetch(next, nsp.index < 0 ? 0 : nlen);
+    }
+    if (fresh) {
+      const float *from = sp.index < 0 ? nullptr
+                          : sp.start < pos ? (OUT ? p.carry + ((int64_t)sec * p.heads + head) * per_state : nullptr)
+                          : p.state_in ? p.state_in + ((int64_t)sp.index * p.heads + head) * per_state : nullptr;
+      has = from != nullptr;
+      if (has) {
+        const bool own = sp.start < pos;  // a carry lies as this walk left it
+        state_load(st, from, kd, vd, !own && p.transposed, own ? 1.f : p.in_by);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) st[t] = zero16();
+      }
+    }
+    if (OUT) {
+      f32x16 acc[2] = {zero16(), zero16()};
+      if (has) {
+#pragma unroll
+        for (int b = 0; b < D / 16; ++b) {
+          const Frag<T> sf = operand<T>(st[b >> 1], b & 1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[i] = mma(sf, row_frag<D>(qt, i * 32 + l31, 16 * b + h8), acc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[i][x] *= into[i];
+      }
+      if (sp.index >= 0) {
+        f32x16 s00 = zero16(), s01 = zero16(), s11 = zero16();  // [key half][row half]
+#pragma unroll
+        for (int b = 0; b < D / 16; ++b) {
+          const Frag<T> k0 = row_frag<D>(kt, pi_of(l31), 16 * b + h8), q0 = row_frag<D>(qt, l31, 16 * b + h8);
+          s00 = mma(k0, q0, s00);
+          if (len > 32) {
+            const Frag<T> k1 = row_frag<D>(kt, 32 + pi_of(l31), 16 * b + h8), q1 = row_frag<D>(qt, 32 + l31, 16 * b + h8);
+            s01 = mma(k0, q1, s01);
+            s11 = mma(k1, q1, s11);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const bool on = 16 * (x >> 3) + h8 + (x & 7) <= l31;
+          s00[x] = on ? s00[x] * wd[x] : 0.f;
+          s11[x] = on ? s11[x] * wd[x] : 0.f;
+          s01[x] *= wo[x];
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          Frag<T> v0 = col_frag<D>(vt, 16 * b, strip);
+          if (dirty) v0 = cleaned(v0);
+          acc[0] = mma(v0, operand<T>(s00, b), acc[0]);
+          if (len > 32) {
+            Frag<T> v1 = col_frag<D>(vt, 32 + 16 * b, strip);
+            if (dirty) v1 = cleaned(v1);
+            acc[1] = mma(v0, operand<T>(s01, b), acc[1]);
+            acc[1] = mma(v1, operand<T>(s11, b), acc[1]);
+          }
+        }
+        if (dirty)  // values that are not finite reach the rows at and behind their own, as NaN
+#pragma unroll 1
+          for (int j = 0; j < len; ++j) {
+            int at = j;
+            asm volatile("" : "+v"(at));  // keeps the addresses below out of the registers of the main path
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const float y = tile_elem<T, D>(vt, at, strip + 16 * (x >> 3) + h8 + (x & 7));
+                if (j <= i * 32 + l31 && !finite(y)) acc[i][x] += y - y;
+                if ((x & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+              }
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 32 + l31;
+        if (r >= len) continue;
+        const int64_t row = p.reverse ? (int64_t)p.s.n - 1 - (pos + r) : pos + r;
+        T *o = (T *)p.out.p + (int64_t)head * p.out.head + row * p.out.row;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc[i][x] *= p.scale;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) store8(o, strip + 16 * b + h8, p.out.dim, p.out.vec, operand<T>(acc[i], b));
+      }
+    }
+    const bool ends = next >= sp.end;
+    if (sp.index >= 0 && (!ends || p.state_out)) {
+      const float fade = power(ld, len);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) st[t][x] *= fade;
+#pragma unroll
+      for (int b = 0; b < DA_PIECE / 16; ++b) {
+        if (16 * b >= len) break;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int left = len - 1 - (16 * b + h8 + e);
+          w[e] = left >= 0 ? power(ld, left + post) : 0.f;
+        }
+        state_add<D>(st, kt, b, w, col_frag<D>(vt, 16 * b, strip), p.state_out != nullptr);
+      }
+      has = true;
+      if (OUT && ends)
+        state_store(st, p.state_out + ((int64_t)sp.index * p.heads + head) * per_state, kd, vd, p.transposed, p.out_by);
+    }
+    fresh = ends;
+    if (next >= sec1) break;
+    pos = next;
+    len = nlen;
+    sp = nsp;
+  }
+  if (!OUT) state_store(st, p.carry + ((int64_t)(sec + 1) * p.heads + head) * per_state, kd, vd, false, 1.f);
+}
+
+// carry[s] holds what section s - 1 adds; link[s] = 2: all of that section is the one series that goes on
+// into s, so that the state before it goes on too, lambda^section times.
+__global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int64_t per_head) {
+  const int64_t blocks = (per_head + 255) / 256;
+  const int head = (int)(blockIdx.x / blocks);
+  const int64_t e = (blockIdx.x % blocks) * 256 + threadIdx.x;
+  if (e >= per_head) return;
+  const float fade = power(p.log_decay[head] * kLog2e, p.section);
+  float *c = p.carry + (int64_t)head * per_head + e;
+  const int64_t step = (int64_t)p.heads * per_head;
+  float x = 0.f;
+  constexpr int AHEAD = 8;
+  for (int s = 1; s < p.sections; s += AHEAD) {
+    float add[AHEAD];
+    int link[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      link[a] = s + a < p.sections ? p.link[s + a] : 0;
+      add[a] = link[a] ? c[(s + a) * step] : 0.f;
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (link[a] == 2) {
+        x = __builtin_fmaf(fade, x, add[a]);
+        c[(s + a) * step] = x;
+      } else {
+        x = add[a];
+      }
+    }
+  }
+}
+
+// A series without rows keeps its state.
+__global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t per_series) {
+  const int s = blockIdx.x;
+  int64_t a = 0, b = p.s.n;
+  if (p.s.offsets) { a = p.s.offsets[s]; b = p.s.offsets[s + 1]; }
+  if (b > p.s.n) b = p.s.n;
+  if (a < 0) a = 0;
+  if (a < b) return;
+  for (int64_t e = threadIdx.x; e < per_series; e += 256)
+    p.state_out[s * per_series + e] = p.state_in ? p.state_in[s * per_series + e] : 0.f;
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+// Sections: some 1024 blocks for the 256 compute units (two to four fit one at a time), whole pieces.
+static int decay_section(int64_t n, int heads) {
+  int64_t s = (n * heads + 1023) / 1024;
+  if (s > n) s = n;
+  s = (s + DA_PIECE - 1) / DA_PIECE * DA_PIECE;
+  if (s < DA_PIECE) s = DA_PIECE;
+  return (int)s;
+}
+
+struct DecayPlan {
+  float *carry;
+  int32_t *link;
+  int section, sections;
+};
+static void decay_plan(const tmp_decay_attention_args *a, Workspace &ws, DecayPlan *d) {
+  const int64_t n = a->n > 0 ? a->n : 1;
+  d->section = decay_section(n, a->heads);
+  d->sections = (int)((n + d->section - 1) / d->section);
+  d->carry = ws.take<float>((size_t)d->sections * a->heads * a->dim_k * a->dim_v);
+  d->link = ws.take<int32_t>(d->sections + 1);
+}
+
+static int decay_check(const tmp_decay_attention_args *a, const char *what, bool grad) {
+  TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
+  TMP_REQUIRE(a->n >= 0 && a->n < (1ll << 31) - 65536, TMP_EINVAL, "%s: row count must be in [0, 2^31 - 65536)", what);
+  TMP_REQUIRE(a->n_series >= 0 && (a->offsets || a->n_series <= 1), TMP_EINVAL, "%s: bad series", what);
+  TMP_REQUIRE(a->type == TMP_BF16 || a->type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
+  TMP_REQUIRE(a->heads > 0 && a->heads <= 65536, TMP_EINVAL, "%s: heads must be in [1, 65536]", what);
+  TMP_REQUIRE(a->dim_k > 0 && a->dim_v > 0, TMP_EINVAL, "%s: head sizes must be positive", what);
+  TMP_REQUIRE(a->dim_k <= TMP_MAX_HEAD_DIM && a->dim_v <= TMP_MAX_HEAD_DIM, TMP_EUNSUPPORTED,
+              "%s: head sizes are limited to %d", what, TMP_MAX_HEAD_DIM);
+  TMP_REQUIRE(a->scale > 0.f && a->scale < INFINITY, TMP_EINVAL, "%s: scale must be positive and finite", what);
+  if (a->n == 0) return TMP_OK;
+  TMP_REQUIRE(a->log_decay && a->q.p && a->k.p && a->v.p, TMP_EINVAL, "%s: null pointer", what);
+  if (grad) TMP_REQUIRE(a->dout.p && a->dq.p && a->dk.p && a->dv.p, TMP_EINVAL, "%s: null pointer", what);
+  else TMP_REQUIRE(a->out.p, TMP_EINVAL, "%s: null pointer", what);
+  return TMP_OK;
+}
+
+template <typename T, int D> static int decay_walk(const DecayParams &p, hipStream_t st) {
+  const int threads = D * 2, piece = DA_PIECE * D * (int)sizeof(T);
+  if (p.sections > 1) {
+    {
+      ProfScope ps("decay_walk_kernel(states)", st);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, false>), dim3((p.sections - 1) * p.heads), dim3(threads),
+                         2 * piece, st, p);
+    }
+    const int64_t per_head = (int64_t)p.k.dim * p.v.dim;
+    TMP_LAUNCH(decay_scan_kernel, dim3((unsigned)((per_head + 255) / 256 * p.heads)), dim3(256), st, p, per_head);
+  }
+  ProfScope ps("decay_walk_kernel", st);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, true>), dim3(p.sections * p.heads), dim3(threads), 3 * piece, st, p);
+  return TMP_OK;
+}
+
+static int decay_run(const DecayParams &p, int type, hipStream_t st) {
+  const int d = padded_dim(p.k.dim > p.v.dim ? p.k.dim : p.v.dim);
+  if (type == TMP_F32)
+    return d == 32 ? decay_walk<float, 32>(p, st) : d == 64 ? decay_walk<float, 64>(p, st) : decay_walk<float, 128>(p, st);
+  return d == 32 ? decay_walk<__bf16, 32>(p, st) : d == 64 ? decay_walk<__bf16, 64>(p, st) : decay_walk<__bf16, 128>(p, st);
+}
+
+static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d) {
+  DecayParams p;
+  memset(&p, 0, sizeof(p));
+  p.s.offsets = a->offsets; p.s.n_series = a->offsets ? a->n_series : 1; p.s.n = (int32_t)a->n;
+  p.log_decay = a->log_decay;
+  p.carry = d.carry; p.link = d.link; p.section = d.section; p.sections = d.sections;
+  p.heads = a->heads; p.scale = a->scale; p.in_by = 1.f; p.out_by = 1.f;
+  return p;
+}
+
+static int decay_empty(const DecayParams &p, int64_t n_series, int64_t per_series, hipStream_t st) {
+  if (p.state_out && n_series > 0)
+    TMP_LAUNCH(decay_empty_kernel, dim3((unsigned)n_series), dim3(256), st, p, per_series);
+  return TMP_OK;
+}
+
+}  // namespace tmp
+
+using namespace tmp;
+
+extern "C" size_t tmp_decay_attention_workspace_bytes(const tmp_decay_attention_args *a) {
+  if (!a || a->heads < 1 || a->dim_k < 1 || a->dim_v < 1) return 0;
+  Workspace ws(nullptr, 0);
+  DecayPlan d;
+  decay_plan(a, ws, &d);
+  return ws.off;
+}
+
+extern "C" int tmp_decay_attention(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream) {
+  clear_error();
+  TMP_TRY(decay_check(a, "tmp_decay_attention", false));
+  Workspace ws(workspace, workspace_bytes);
+  DecayPlan d;
+  decay_plan(a, ws, &d);
+  TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_decay_attention: workspace too small");
+  hipStream_t st = (hipStream_t)stream;
+  const int b = a->type == TMP_F32 ? 4 : 2;
+  DecayParams p = decay_params(a, d);
+  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b);
+  p.v = rows_of(a->v, a->dim_v, b); p.out = rows_of(a->out, a->dim_v, b);
+  p.state_in = a->state_in; p.state_out = a->state_out;
+  if (a->n > 0) TMP_TRY(decay_run(p, a->type, st));
+  TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
+  TMP_CHECK_HIP(hipGetLastError());
+  return TMP_OK;
+}
+
+extern "C" int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream) {
+  clear_error();
+  TMP_TRY(decay_check(a, "tmp_decay_attention_grad", true));
+  Workspace ws(workspace, workspace_bytes);
+  DecayPlan d;
+  decay_plan(a, ws, &d);
+  TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_decay_attention_grad: workspace too small");
+  hipStream_t st = (hipStream_t)stream;
+  const int b = a->type == TMP_F32 ? 4 : 2;
+  const Rows q = rows_of(a->q, a->dim_k, b), k = rows_of(a->k, a->dim_k, b), v = rows_of(a->v, a->dim_v, b);
+  const Rows o = rows_of(a->dout, a->dim_v, b);
+  DecayParams p = decay_params(a, d);
+  if (a->n > 0) {
+    p.q = o; p.k = v; p.v = k; p.out = rows_of(a->dq, a->dim_k, b);
+    p.state_in = a->state_in; p.transposed = 1;
+    TMP_TRY(decay_run(p, a->type, st));
+  }
+  p.reverse = 1; p.state_in = a->dstate_out; p.in_by = 1.f / a->scale; p.out_by = a->scale;
+  if (a->n > 0) {
+    p.q = v; p.k = o; p.v = q; p.out = rows_of(a->dk, a->dim_k, b);
+    TMP_TRY(decay_run(p, a->type, st));
+    p.q = k; p.k = q; p.v = o; p.out = rows_of(a->dv, a->dim_v, b);
+    p.transposed = 0; p.state_out = a->dstate_in;
+    TMP_TRY(decay_run(p, a->type, st));
+  }
+  p.state_out = a->dstate_in;
+  TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
+  TMP_CHECK_HIP(hipGetLastError());
+  return TMP_OK;
+}

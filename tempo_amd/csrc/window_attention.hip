@@ -1,0 +1,642 @@
+// Attention over a sliding window of each series, with a few first rows that stay visible.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  lse_i = log sum_j exp(scale q_i.k_j)
+//   j of i's series with j <= i and (j > i - window or j < start + sinks)
+//
+// and backward, with dP_ij = do_i.v_j and dS_ij = p_ij (dP_ij - do_i.o_i):
+//   dq_i = scale sum_j dS_ij k_j    dk_j = scale sum_i dS_ij q_i    dv_j = sum_i p_ij do_i
+//
+// One skeleton serves all three kernels: a wave owns 32 rows, one per column of the matrix cores'
+// result (its operands of them stay in registers), and the block's four waves stream the other side's
+// rows through LDS in tiles of 64.  A row's scores then lie in two lanes, so the running maximum and
+// sum of the softmax are lane-local but for one exchange, and scores turn into operands in place.
+#include <string.h>
+
+#include "series_tile.h"
+
+namespace tmp {
+
+constexpr int WA_OWN = 128;    // rows that a block owns, 32 to each wave
+constexpr int WA_TILE = 64;    // rows of a streamed tile
+constexpr int WA_THREADS = 256;
+constexpr int WA_SECTION = 256;  // rows whose share of the sinks' gradients is added up by one block
+
+struct WindowParams {
+  Series s;
+  Rows q, k, v, out, dout, dq, dk, dv;
+  float *lse;    // [n][heads]
+  float *delta;  // [n][heads], do_i.o_i
+  float *sink_part;  // [sections][2][kv_heads][sinks][dk + dv]
+  int32_t heads, kv_heads, window, sinks;
+  float scale;
+};
+
+struct Seen {  // which rows j a row i sees
+  int window, sinks;
+  __device__ inline bool operator()(int i, int j, int start) const {
+    return j <= i && j >= start && (j > i - window || j < start + sinks);
+  }
+};
+
+// What a wave knows of its 32 own rows when they are query rows.
+struct QueryRows {
+  int i, start;               // the lane's row and where its series starts (i + 1: none)
+  int lo, first_start;        // of the block: first row in any window, start of its first row's series
+  int wmin, wmax, wlo, wstart;  // of the wave: first and last row, first row in any window, last start
+  bool all;                   // every row of the wave lies in a series
+};
+
+__device__ inline QueryRows query_rows(const WindowParams &p, int t0) {
+  QueryRows r;
+  const int t1 = t0 + WA_OWN < p.s.n ? t0 + WA_OWN : p.s.n;
+  const int most = p.s.n_series + 1;
+  const int c0 = count_le(p.s, t0, 0, most);
+  int c1 = c0;
+  if (p.s.offsets && c0 < most && p.s.offsets[c0] < t1) c1 = count_le(p.s, t1 - 1, c0, most);
+  r.i = t0 + (threadIdx.x >> 6) * 32 + (lane_id() & 31);
+  const Span first = span_at(p.s, c0, t0);
+  r.first_start = first.start < t0 ? first.start : t0;
+  const int w = t0 - p.window + 1;
+  r.lo = w > r.first_start ? w : r.first_start;
+  Span mine = first;
+  bool in = r.i < t1;
+  if (c1 != c0 && in) mine = span_at(p.s, count_le_lane(p.s, r.i, c0, c1), r.i);
+  in = in && mine.start <= r.i;
+  r.start = in ? mine.start : r.i + 1;
+  r.wmin = t0 + (threadIdx.x >> 6) * 32;
+  r.wmax = r.wmin + 31;
+  const int lo = r.i - p.window + 1 > r.start ? r.i - p.window + 1 : r.start;
+  r.wlo = wave_min(lo);
+  r.wstart = wave_max(r.start);
+  r.all = __all(in);
+  return r;
+}
+
+// The tiles of rows that query rows look at: the first series' sinks that lie before every window
+// (part 0), then all rows from the first window on (part 1).
+struct KeyTiles {
+  int a0, a1, b0, b1, na, count;
+  __device__ inline KeyTiles(const WindowParams &p, const QueryRows &r, int t0) {
+    a0 = r.first_start;
+    a1 = a0 + p.sinks < r.lo ? a0 + p.sinks : r.lo;
+    if (a1 < a0) a1 = a0;
+    b0 = r.lo;
+    b1 = t0 + WA_OWN < p.s.n ? t0 + WA_OWN : p.s.n;
+    na = (a1 - a0 + WA_TILE - 1) / WA_TILE;
+    count = na + (b1 - b0 + WA_TILE - 1) / WA_TILE;
+  }
+  __device__ inline int first(int t) const { return t < na ? a0 + t * WA_TILE : b0 + (t - na) * WA_TILE; }
+  __device__ inline int end(int t) const { return t < na ? a1 : b1; }
+  __device__ inline int rows(int t) const {
+    const int left = end(t) - first(t);
+    return left < WA_TILE ? left : WA_TILE;
+  }
+};
+
+// Adds what the products left out: streamed values that are not finite and visible.  nan: as NaN (the
+// factor may be zero or have either sign), else as they are (the factor is a positive weight).
+template <typename T, int D, int NT, typename F>
+__device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, int row0, bool nan, F seen) {
+  const int h8 = (lane_id() >> 5) * 8;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    if (!seen(j)) continue;
+    int row = row0 + j;
+    asm volatile("" : "+v"(row));  // keeps the addresses below out of the registers of the main path
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float x = tile_elem<T, D>(tile, row, t * 32 + 16 * (r >> 3) + h8 + (r & 7));
+        if (!finite(x)) acc[t][r] += nan ? x - x : x;
+        if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+}
+
+template <typename T, int D>
+__device__ inline void load_own(Frag<T> (&f)[D / 16], const Rows &rows, int head, int row, bool in) {
+  const T *p = head_of<T>(rows, head) + (int64_t)row * rows.row;
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b)
+    f[b] = in ? load8(p, 16 * b + 8 * (lane_id() >> 5), rows.dim, rows.vec) : zero_frag<Frag<T>>();
+}
+template <typename T, int D, int NT>
+__device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &rows, int head, int row, bool in) {
+  if (!in) return;
+  T *p = (T *)rows.p + (int64_t)head * rows.head + (int64_t)row * rows.row;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    f32x16 c = acc[t];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[r] *= by;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) store8(p, t * 32 + 16 * b + 8 * (lane_id() >> 5), rows.dim, rows.vec, operand<T>(c, b));
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_forward_kernel(WindowParams p, int tiles) {
+  const int item = item_of_block(tiles * p.heads);
+  if (item < 0) return;
+  const int group = p.heads / p.kv_heads;
+  const int kv = item / (tiles * group), rest = item % (tiles * group);
+  const int t0 = rest / group * WA_OWN, head = kv * group + rest % group;
+  __shared__ __align__(16) T kt[WA_TILE * D], vt[WA_TILE * D];
+  __shared__ int flag[2];
+  if (threadIdx.x < 2) flag[threadIdx.x] = 0;
+  const QueryRows r = query_rows(p, t0);
+  const KeyTiles tl(p, r, t0);
+  const Seen seen = {p.window, p.sinks};
+  const int h8 = (lane_id() >> 5) * 8;
+  const bool in = r.start <= r.i;
+  Frag<T> qf[D / 16];
+  load_own<T, D>(qf, p.q, head, r.i, in);
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale * kLog2e;
+  const T *kp = head_of<T>(p.k, kv), *vp = head_of<T>(p.v, kv);
+  Staged<T, D, WA_TILE, WA_THREADS> ks, vs;
+  ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(0), 1, tl.rows(0));
+  vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(0), 1, tl.rows(0));
+  for (int t = 0; t < tl.count; ++t) {
+    const int j0 = tl.first(t), j1 = tl.end(t);
+    __syncthreads();
+    ks.store(kt);
+    if (vs.store(vt)) flag[t & 1] = 1;
+    if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
+    __syncthreads();
+    if (t + 1 < tl.count) {
+      ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+      vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+    }
+    const bool dirty = flag[t & 1];
+    if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;  // none of the wave's
+    const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
+    // (rows behind part 0 are part 1's)
+    auto visible = [&](int j) { return j < j1 && seen(r.i, j, r.start); };
+    f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b)
+        s[u] = mma(row_frag<D>(kt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
+    if (!full)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (!visible(j0 + u * 32 + 16 * (x >> 3) + h8 + (x & 7))) s[u][x] = -INFINITY;
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+    top = fmaxf(top, other_half(top)) * c;
+    if (__any(top > m)) {
+      const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
+      m = nm;
+      l *= by;
+#pragma unroll
+      for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc[t2][x] *= by;
+    }
+    const float mm = m > -INFINITY ? m : 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
+        l += s[u][x];
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Frag<T> pf = operand<T>(s[u], b);
+#pragma unroll
+        for (int t2 = 0; t2 < D / 32; ++t2) {
+          Frag<T> vf = col_frag<D>(vt, u * 32 + 16 * b, t2 * 32);
+          if (dirty) vf = cleaned(vf);
+          acc[t2] = mma(vf, pf, acc[t2]);
+        }
+      }
+      if (dirty)
+        add_not_finite<T, D>(acc, vt, u * 32, false, [&](int j) { return visible(j0 + u * 32 + j); });
+    }
+  }
+  l += other_half(l);
+  // a row of no series gets zeros
+  const float by = in ? 1.f / l : 0.f;
+  store_own<T, D>(acc, by, p.out, head, r.i, r.i < p.s.n);
+  if (p.lse && r.i < p.s.n && lane_id() < 32)
+    p.lse[(int64_t)r.i * p.heads + head] = in ? (m + log2_hw(l)) * kLn2 : -INFINITY;
+}
+
+// dq, and do.o for the kernel that follows.
+template <typename T, int D>
+__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_dq_kernel(WindowParams p, int tiles) {
+  const int item = item_of_block(tiles * p.heads);
+  if (item < 0) return;
+  const int group = p.heads / p.kv_heads;
+  const int kv = item / (tiles * group), rest = item % (tiles * group);
+  const int t0 = rest / group * WA_OWN, head = kv * group + rest % group;
+  __shared__ __align__(16) T kt[WA_TILE * D], vt[WA_TILE * D];
+  __shared__ int flag[2];
+  if (threadIdx.x < 2) flag[threadIdx.x] = 0;
+  const QueryRows r = query_rows(p, t0);
+  const KeyTiles tl(p, r, t0);
+  const Seen seen = {p.window, p.sinks};
+  const int h8 = (lane_id() >> 5) * 8;
+  const bool in = r.start <= r.i;
+  Frag<T> qf[D / 16], of[D / 16];
+  load_own<T, D>(of, p.out, head, r.i, in);
+  load_own<T, D>(qf, p.dout, head, r.i, in);
+  float delta = 0.f;
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta = __builtin_fmaf((float)of[b][e], (float)qf[b][e], delta);
+  delta += other_half(delta);
+  if (r.i < p.s.n && lane_id() < 32) p.delta[(int64_t)r.i * p.heads + head] = delta;
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b) of[b] = qf[b];
+  load_own<T, D>(qf, p.q, head, r.i, in);
+  const float lse2 = in ? p.lse[(int64_t)r.i * p.heads + head] * kLog2e : 0.f;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
+  const float c = p.scale * kLog2e;
+  const T *kp = head_of<T>(p.k, kv), *vp = head_of<T>(p.v, kv);
+  Staged<T, D, WA_TILE, WA_THREADS> ks, vs;
+  ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(0), 1, tl.rows(0));
+  vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(0), 1, tl.rows(0));
+  for (int t = 0; t < tl.count; ++t) {
+    const int j0 = tl.first(t), j1 = tl.end(t);
+    __syncthreads();
+    if (ks.store(kt)) flag[t & 1] = 1;
+    vs.store(vt);
+    if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
+    __syncthreads();
+    if (t + 1 < tl.count) {
+      ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+      vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+    }
+    const bool dirty = flag[t & 1];
+    if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;
+    const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
+    // (rows behind part 0 are part 1's)
+    auto visible = [&](int j) { return j < j1 && seen(r.i, j, r.start); };
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b) {
+        s = mma(row_frag<D>(kt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s);
+        dp = mma(row_frag<D>(vt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), of[b], dp);
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float w = exp2_hw(__builtin_fmaf(s[x], c, -lse2)) * (dp[x] - delta);
+        s[x] = full || visible(j0 + u * 32 + 16 * (x >> 3) + h8 + (x & 7)) ? w : 0.f;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Frag<T> pf = operand<T>(s, b);
+#pragma unroll
+        for (int t2 = 0; t2 < D / 32; ++t2) {
+          Frag<T> kf = col_frag<D>(kt, u * 32 + 16 * b, t2 * 32);
+          if (dirty) kf = cleaned(kf);
+          acc[t2] = mma(kf, pf, acc[t2]);
+        }
+      }
+      if (dirty)
+        add_not_finite<T, D>(acc, kt, u * 32, true, [&](int j) { return visible(j0 + u * 32 + j); });
+    }
+  }
+  store_own<T, D>(acc, p.scale, p.dq, head, r.i, r.i < p.s.n);
+}
+
+// Last query row + 1 whose pairs with the key rows of tile [j0, j0 + WA_OWN) the main dk/dv kernel adds:
+// the window's, and the section's where the tile holds rows that stay visible.  Pairs of such a row
+// with later rows are the sink kernel's.
+__device__ inline int last_query(const WindowParams &p, int j0, bool sinks) {
+  int64_t hi = (int64_t)j0 + WA_OWN + p.window - 1;
+  const int64_t sec = ((int64_t)j0 / WA_SECTION + 1) * WA_SECTION;
+  if (sinks && sec > hi) hi = sec;
+  return hi < p.s.n ? (int)hi : p.s.n;
+}
+
+// dk and dv: a block owns key rows and streams the query rows that see them, head after head of the
+// group that shares them.  SINK: the rows that stay visible, against the query rows of one section
+// that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
+template <typename T, int D, bool SINK>
+__global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
+  const int item = item_of_block(tiles * p.kv_heads);
+  if (item < 0) return;
+  const int group = p.heads / p.kv_heads;
+  const int kv = item / tiles, tile = item % tiles;
+  const int wave = threadIdx.x >> 6, lane = lane_id(), h8 = (lane >> 5) * 8;
+  __shared__ __align__(16) T qt[WA_TILE * D], dt[WA_TILE * D];
+  __shared__ float lse_t[WA_TILE], delta_t[WA_TILE];
+  __shared__ int flag[2];
+  if (threadIdx.x < 2) flag[threadIdx.x] = 0;
+  const int most = p.s.n_series + 1;
+  int j, start, end, i0, i1, from = 0;  // the lane's key row and its series; query rows [i0, i1), those before `from` left out
+  if (SINK) {
+    const int sec0 = tile * WA_SECTION;
+    const Span sp = span_at(p.s, count_le(p.s, sec0, 0, most), sec0);
+    if (sp.start >= sec0) return;  // (uniform) no series reaches over the section's start
+    j = sp.start + (lane & 31);
+    start = sp.start;
+    end = (lane & 31) < p.sinks && j < sp.end ? sp.end : j;
+    // a row of this kernel's tile of the other form has pairs up to last_query there
+    from = last_query(p, j / WA_OWN * WA_OWN, true);
+    i0 = sec0;
+    i1 = sec0 + WA_SECTION < sp.end ? sec0 + WA_SECTION : sp.end;
+    if (j / WA_SECTION >= tile) from = i1;  // (a sink row inside the section itself: all its pairs are the other form's)
+  } else {
+    const int j0 = tile * WA_OWN, j1 = j0 + WA_OWN < p.s.n ? j0 + WA_OWN : p.s.n;
+    const int c0 = count_le(p.s, j0, 0, most);
+    int c1 = c0;
+    if (p.s.offsets && c0 < most && p.s.offsets[c0] < j1) c1 = count_le(p.s, j1 - 1, c0, most);
+    j = j0 + wave * 32 + (lane & 31);
+    Span mine = span_at(p.s, c0, j0);
+    if (c1 != c0 && j < j1) mine = span_at(p.s, count_le_lane(p.s, j, c0, c1), j);
+    const bool in = j < j1 && mine.start <= j;
+    start = in ? mine.start : j;
+    end = in ? mine.end : j;
+    i0 = j0;
+    // every wave looks at the same rows: the last series' sinks decide for the block
+    const Span last = span_at(p.s, c1, j1 - 1), fst = span_at(p.s, c0, j0);
+    const bool sinks = p.sinks > 0 && (c1 != c0 || fst.start + p.sinks > j0);
+    i1 = last_query(p, j0, sinks);
+    const int reach = last.start <= j1 - 1 ? last.end : j1;
+    if (i1 > reach) i1 = reach > j1 ? reach : j1;
+    if (i1 < j1) i1 = j1;
+  }
+  const Seen seen = {p.window, p.sinks};
+  const bool in = end > j;
+  Frag<T> kf[D / 16], vf[D / 16];
+  load_own<T, D>(kf, p.k, kv, j, in);
+  load_own<T, D>(vf, p.v, kv, j, in);
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) { dk[t] = zero16(); dv[t] = zero16(); }
+  const float c = p.scale * kLog2e;
+  const int per_head = (i1 - i0 + WA_TILE - 1) / WA_TILE, count = per_head * group;
+  Staged<T, D, WA_TILE, WA_THREADS> qs, ds;
+  float lse_n = 0.f, delta_n = 0.f;
+  auto fetch = [&](int t) {
+    const int head = kv * group + t / per_head, first = i0 + t % per_head * WA_TILE;
+    const int rows = i1 - first < WA_TILE ? i1 - first : WA_TILE;
+    qs.load(head_of<T>(p.q, head), p.q.row, p.q.dim, p.q.vec, first, 1, rows);
+    ds.load(head_of<T>(p.dout, head), p.dout.row, p.dout.dim, p.dout.vec, first, 1, rows);
+    if (threadIdx.x < WA_TILE && (int)threadIdx.x < rows) {
+      const int64_t at = (int64_t)(first + threadIdx.x) * p.heads + head;
+      lse_n = p.lse[at] * kLog2e;
+      delta_n = p.delta[at];
+    }
+  };
+  if (count > 0) fetch(0);
+  const int wmin_j = j - (lane & 31), wmax_j = wmin_j + 31;
+  const int wend = wave_max(end), wfrom = wave_min(from);
+  for (int t = 0; t < count; ++t) {
+    const int r0 = i0 + t % per_head * WA_TILE;
+    __syncthreads();
+    bool bad = qs.store(qt);
+    bad |= ds.store(dt) != 0;
+    if (bad) flag[t & 1] = 1;
+    if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
+    if (threadIdx.x < WA_TILE) { lse_t[threadIdx.x] = lse_n; delta_t[threadIdx.x] = delta_n; }
+    __syncthreads();
+    if (t + 1 < count) fetch(t + 1);
+    const bool dirty = flag[t & 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int ru = r0 + u * 32;
+      if (SINK) {
+        if (wave != u || ru + 32 <= wfrom) continue;  // two waves share the section's rows
+      } else {
+        if (ru + 31 < wmin_j || ru >= wend) continue;
+        if (p.sinks == 0 && ru > wmax_j + p.window - 1) continue;
+      }
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int b = 0; b < D / 16; ++b) {
+        s = mma(row_frag<D>(qt, u * 32 + pi_of(lane & 31), 16 * b + h8), kf[b], s);
+        dp = mma(row_frag<D>(dt, u * 32 + pi_of(lane & 31), 16 * b + h8), vf[b], dp);
+      }
+      auto visible = [&](int i) { return i >= from && i < end && i < i1 && seen(i, j, start); };
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int row = u * 32 + 16 * (x >> 3) + h8 + (x & 7);
+        const bool on = visible(r0 + row);
+        const float w = exp2_hw(__builtin_fmaf(s[x], c, -lse_t[row]));
+        const float g = w * (dp[x] - delta_t[row]);
+        s[x] = on ? w : 0.f;
+        dp[x] = on ? g : 0.f;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const Frag<T> pf = operand<T>(s, b), gf = operand<T>(dp, b);
+#pragma unroll
+        for (int t2 = 0; t2 < D / 32; ++t2) {
+          Frag<T> of = col_frag<D>(dt, u * 32 + 16 * b, t2 * 32), qf = col_frag<D>(qt, u * 32 + 16 * b, t2 * 32);
+          if (dirty) { of = cleaned(of); qf = cleaned(qf); }
+          dv[t2] = mma(of, pf, dv[t2]);
+          dk[t2] = mma(qf, gf, dk[t2]);
+        }
+      }
+      if (dirty) {
+        add_not_finite<T, D>(dv, dt, u * 32, false, [&](int x) { return visible(ru + x); });
+        add_not_finite<T, D>(dk, qt, u * 32, true, [&](int x) { return visible(ru + x); });
+      }
+    }
+  }
+  if (SINK) {
+    if (wave > 1 || (lane & 31) >= p.sinks) return;
+    const int width = p.k.dim + p.v.dim;
+    float *o = p.sink_part + ((((int64_t)tile * 2 + wave) * p.kv_heads + kv) * p.sinks + (lane & 31)) * width;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int d = t * 32 + 16 * (x >> 3) + h8 + (x & 7);
+        if (d < p.k.dim) o[d] = dk[t][x];
+        if (d < p.v.dim) o[p.k.dim + d] = dv[t][x];
+      }
+    return;
+  }
+  if (p.sinks > 0 && in && j < start + p.sinks && (end - 1) / WA_SECTION > start / WA_SECTION) {
+    // what the sections behind the series' first add, summed up in the place of the first of them
+    const int width = p.k.dim + p.v.dim;
+    const float *o = p.sink_part + (((int64_t)(start / WA_SECTION + 1) * 2 * p.kv_heads + kv) * p.sinks + (j - start)) * width;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int d = t * 32 + 16 * (x >> 3) + h8 + (x & 7);
+        if (d < p.k.dim) dk[t][x] += o[d];
+        if (d < p.v.dim) dv[t][x] += o[p.k.dim + d];
+      }
+  }
+  store_own<T, D>(dk, p.scale, p.dk, kv, j, j < p.s.n);
+  store_own<T, D>(dv, 1.f, p.dv, kv, j, j < p.s.n);
+}
+
+// Adds up the parts of all sections that a series reaches into, in the place of the first of them.  A
+// block takes one (section, key/value head) and has work only where the section is such a first one.
+__global__ __launch_bounds__(256) void sink_sum_kernel(WindowParams p) {
+  const int sec = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
+  const int sec0 = sec * WA_SECTION;
+  const Span sp = span_at(p.s, count_le(p.s, sec0, 0, p.s.n_series + 1), sec0);
+  if (sp.start >= sec0 || sp.start / WA_SECTION + 1 != sec) return;
+  const int last = (sp.end - 1) / WA_SECTION;
+  const int count = p.sinks * (p.k.dim + p.v.dim);
+  const int64_t step = (int64_t)p.kv_heads * count;  // from one part to the next
+  float *o = p.sink_part + ((int64_t)sec * 2 * p.kv_heads + kv) * count;
+  for (int e = threadIdx.x; e < count; e += 256) {
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int parts = (last - sec + 1) * 2;
+    int a = 0;
+    for (; a + 8 <= parts; a += 8)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) sum[x] += o[(a + x) * step + e];
+    for (; a < parts; ++a) sum[0] += o[a * step + e];
+    o[e] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+static int window_check(const tmp_window_attention_args *a, const char *what, bool grad) {
+  TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
+  TMP_REQUIRE(a->n >= 0 && a->n < (1ll << 31) - 65536, TMP_EINVAL, "%s: row count must be in [0, 2^31 - 65536)", what);
+  TMP_REQUIRE(a->n_series >= 0 && (a->offsets || a->n_series <= 1), TMP_EINVAL, "%s: bad series", what);
+  TMP_REQUIRE(a->type == TMP_BF16 || a->type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
+  TMP_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 65536, TMP_EINVAL,
+              "%s: heads (%d) must be a multiple of kv_heads (%d), at most 65536", what, a->heads, a->kv_heads);
+  TMP_REQUIRE(a->dim_k > 0 && a->dim_v > 0, TMP_EINVAL, "%s: head sizes must be positive", what);
+  TMP_REQUIRE(a->dim_k <= TMP_MAX_HEAD_DIM && a->dim_v <= TMP_MAX_HEAD_DIM, TMP_EUNSUPPORTED,
+              "%s: head sizes are limited to %d", what, TMP_MAX_HEAD_DIM);
+  TMP_REQUIRE(a->window >= 1, TMP_EINVAL, "%s: window must be >= 1", what);
+  TMP_REQUIRE(a->scale > 0.f && a->scale < INFINITY, TMP_EINVAL, "%s: scale must be positive and finite", what);
+  TMP_REQUIRE(a->sinks >= 0, TMP_EINVAL, "%s: sinks must be >= 0", what);
+  TMP_REQUIRE(a->sinks <= TMP_MAX_SINKS, TMP_EUNSUPPORTED, "%s: at most %d sinks", what, TMP_MAX_SINKS);
+  TMP_REQUIRE((a->n + WA_OWN - 1) / WA_OWN * a->heads < (1ll << 31) - 64, TMP_EUNSUPPORTED, "%s: too many rows x heads", what);
+  if (a->n == 0) return TMP_OK;
+  TMP_REQUIRE(a->q.p && a->k.p && a->v.p && a->out.p, TMP_EINVAL, "%s: null pointer", what);
+  if (grad)
+    TMP_REQUIRE(a->dout.p && a->dq.p && a->dk.p && a->dv.p && a->lse, TMP_EINVAL, "%s: null pointer", what);
+  return TMP_OK;
+}
+
+static WindowParams window_params(const tmp_window_attention_args *a) {
+  WindowParams p;
+  memset(&p, 0, sizeof(p));
+  const int b = a->type == TMP_F32 ? 4 : 2;
+  p.s.offsets = a->offsets; p.s.n_series = a->n_series; p.s.n = (int32_t)a->n;
+  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b); p.v = rows_of(a->v, a->dim_v, b);
+  p.out = rows_of(a->out, a->dim_v, b); p.dout = rows_of(a->dout, a->dim_v, b);
+  p.dq = rows_of(a->dq, a->dim_k, b); p.dk = rows_of(a->dk, a->dim_k, b); p.dv = rows_of(a->dv, a->dim_v, b);
+  p.lse = a->lse;
+  p.heads = a->heads; p.kv_heads = a->kv_heads; p.sinks = a->sinks; p.scale = a->scale;
+  p.window = (int32_t)(a->window < a->n ? a->window : a->n);
+  return p;
+}
+
+template <typename T, int D> static void window_forward(const WindowParams &p, hipStream_t st) {
+  const int tiles = (p.s.n + WA_OWN - 1) / WA_OWN;
+  ProfScope ps("window_forward_kernel", st);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_forward_kernel<T, D>), dim3(grid_of_items((int64_t)tiles * p.heads)),
+                     dim3(WA_THREADS), 0, st, p, tiles);
+}
+
+template <typename T, int D> static void window_grad(const WindowParams &p, hipStream_t st) {
+  const int tiles = (p.s.n + WA_OWN - 1) / WA_OWN, sections = (p.s.n + WA_SECTION - 1) / WA_SECTION;
+  {
+    ProfScope ps("window_dq_kernel", st);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dq_kernel<T, D>), dim3(grid_of_items((int64_t)tiles * p.heads)),
+                       dim3(WA_THREADS), 0, st, p, tiles);
+  }
+  if (p.sinks > 0 && sections > 1) {
+    {
+      ProfScope ps("window_dkdv_kernel(sinks)", st);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, true>), dim3(grid_of_items((int64_t)sections * p.kv_heads)),
+                         dim3(WA_THREADS), 0, st, p, sections);
+    }
+    TMP_LAUNCH(sink_sum_kernel, dim3(sections * p.kv_heads), dim3(256), st, p);
+  }
+  ProfScope ps("window_dkdv_kernel", st);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, false>), dim3(grid_of_items((int64_t)tiles * p.kv_heads)),
+                     dim3(WA_THREADS), 0, st, p, tiles);
+}
+
+struct WindowPlan {
+  float *delta, *sink_part;
+};
+static void window_plan(const tmp_window_attention_args *a, Workspace &ws, WindowPlan *w) {
+  const int64_t n = a->n > 0 ? a->n : 1;
+  w->delta = ws.take<float>((size_t)n * a->heads);
+  const int64_t sections = (n + WA_SECTION - 1) / WA_SECTION;
+  w->sink_part = ws.take<float>(a->sinks > 0 && sections > 1
+                                    ? (size_t)sections * 2 * a->kv_heads * a->sinks * (a->dim_k + a->dim_v) : 1);
+}
+
+#define TMP_BY_TYPE_AND_DIM(fn, type, d, ...)                                        \
+  do {                                                                               \
+    if ((type) == TMP_F32) {                                                         \
+      if ((d) == 32) fn<float, 32>(__VA_ARGS__);                                     \
+      else if ((d) == 64) fn<float, 64>(__VA_ARGS__);                                \
+      else fn<float, 128>(__VA_ARGS__);                                              \
+    } else {                                                                         \
+      if ((d) == 32) fn<__bf16, 32>(__VA_ARGS__);                                    \
+      else if ((d) == 64) fn<__bf16, 64>(__VA_ARGS__);                               \
+      else fn<__bf16, 128>(__VA_ARGS__);                                             \
+    }                                                                                \
+  } while (0)
+
+}  // namespace tmp
+
+using namespace tmp;
+
+extern "C" int tmp_window_attention(const tmp_window_attention_args *a, void *stream) {
+  clear_error();
+  TMP_TRY(window_check(a, "tmp_window_attention", false));
+  if (a->n == 0) return TMP_OK;
+  const WindowParams p = window_params(a);
+  const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
+  TMP_BY_TYPE_AND_DIM(window_forward, a->type, d, p, (hipStream_t)stream);
+  TMP_CHECK_HIP(hipGetLastError());
+  return TMP_OK;
+}
+
+extern "C" size_t tmp_window_attention_grad_workspace_bytes(const tmp_window_attention_args *a) {
+  if (!a || window_check(a, "tmp_window_attention_grad", false) != TMP_OK) return 0;
+  Workspace ws(nullptr, 0);
+  WindowPlan w;
+  window_plan(a, ws, &w);
+  return ws.off;
+}
+
+extern "C" int tmp_window_attention_grad(const tmp_window_attention_args *a, void *workspace, size_t workspace_bytes,
+                                         void *stream) {
+  clear_error();
+  TMP_TRY(window_check(a, "tmp_window_attention_grad", true));
+  if (a->n == 0) return TMP_OK;
+  WindowParams p = window_params(a);
+  Workspace ws(workspace, workspace_bytes);
+  WindowPlan w;
+  window_plan(a, ws, &w);
+  TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_window_attention_grad: workspace too small");
+  p.delta = w.delta;
+  p.sink_part = w.sink_part;
+  const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
+  TMP_BY_TYPE_AND_DIM(window_grad, a->type, d, p, (hipStream_t)stream);
+  TMP_CHECK_HIP(hipGetLastError());
+  return TMP_OK;
+}

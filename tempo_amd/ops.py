@@ -814,3 +814,8 @@ def write_layout(key, ts, n_keys):
     check(lib().tmp_write_layout(C.byref(a), ws.data_ptr(), ws.numel(), _stream()),
           "tmp_write_layout")
     return event_dt, event_time, perm, dt_range
+
+
+# attention over ordered series (tempo_amd/attention.py)
+from .attention import (decay_attention, decay_attention_grad, decay_attention_step, series_offsets,  # noqa: E402,F401
+                        window_attention, window_attention_grad, window_attention_step, window_cache_write)
