@@ -107,10 +107,10 @@ __device__ inline int place_of(int64_t t, int sinks, int window) {
 }
 
 // A wave takes `chunk` rows of one slot's cache, one key/value head and up to 32 of its query heads.
-template <typename T, int D>
+template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(256, D * sizeof(T) >= 512 ? 1 : 2) void window_step_kernel(WindowStepParams p, int units) {
   extern __shared__ __align__(16) unsigned char smem[];
-  const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   if (unit >= units) return;
   T *vt = (T *)smem + (threadIdx.x >> 6) * 32 * D;
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8;
@@ -128,52 +128,50 @@ __global__ __launch_bounds__(256, D * sizeof(T) >= 512 ? 1 : 2) void window_step
   const int head = kv * group + part * 32 + l31;
   const bool on = part * 32 + l31 < group;
   float *out = p.part + (((int64_t)b * p.heads + (on ? head : kv * group)) * p.splits + split) * (p.v.dim + 2);
-  const T *kn = head_of<T>(p.k, kv) + (int64_t)b * p.k.row, *vn = head_of<T>(p.v, kv) + (int64_t)b * p.v.row;
-  T *kc = (T *)p.kc.p + slot * p.kc_slot + kv * p.kc.head, *vc = (T *)p.vc.p + slot * p.vc_slot + kv * p.vc.head;
-  Frag<T> qf[D / 16];
-  {
-    const T *qp = head_of<T>(p.q, on ? head : 0) + (int64_t)b * p.q.row;
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x) qf[x] = on ? load8(qp, 16 * x + h8, p.q.dim, p.q.vec) : zero_frag<Frag<T>>();
-  }
-  // the new row goes into the cache; nobody reads its place there in this call
-  if (part == 0 && place >= r0 && place < r1)
+  Rows kc = p.kc, vc = p.vc;
+  kc.p = (T *)p.kc.p + slot * p.kc_slot;
+  vc.p = (T *)p.vc.p + slot * p.vc_slot;
+  // The new row goes into the cache first.  Only the waves whose rows hold its place read that place (waves of
+  // the same rows and other query heads write the same there), each behind its own write.
+  if (place >= r0 && place < r1) {
+    const T *kn = head_of<T>(p.k, kv) + (int64_t)b * p.k.row, *vn = head_of<T>(p.v, kv) + (int64_t)b * p.v.row;
+    T *ko = (T *)head_of<T>(kc, kv) + (int64_t)place * kc.row, *vo = (T *)head_of<T>(vc, kv) + (int64_t)place * vc.row;
     for (int d = lane; d < TMP_MAX_HEAD_DIM; d += 64) {
-      if (d < p.k.dim) kc[(int64_t)place * p.kc.row + d] = kn[d];
-      if (d < p.v.dim) vc[(int64_t)place * p.vc.row + d] = vn[d];
+      if (d < p.k.dim) ko[d] = kn[d];
+      if (d < p.v.dim) vo[d] = vn[d];
+    }
+    __threadfence_block();
+  }
+  Frag<T> qf[D / 16];
+  const T *qp = head_of<T>(p.q, on ? head : 0) + (int64_t)b * p.q.row;
+#pragma unroll
+  for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = 16 * x + h8 + e;
+      qf[x][e] = on && d < p.q.dim ? qp[d] : (T)0.f;
     }
   f32x16 acc[D / 32];
 #pragma unroll
   for (int x = 0; x < D / 32; ++x) acc[x] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * kLog2e;
-  Frag<T> kf[D / 16], vf[D / 16];
+  Frag<T> kf[D / 16];
+  Staged<T, D, 32, 64, VEC> vs;
   auto fetch = [&](int row0) {
-    const int row = row0 + pi_of(l31);
-    const T *kp = row == place ? kn : kc + (int64_t)row * p.kc.row;
-    const bool kvec = row == place ? p.k.vec : p.kc.vec;
+    const int rows = r1 - row0 < 32 ? r1 - row0 : 32;
+    const Run kb = rows_buffer<T>(kc, kv, row0, rows);
+    const uint32_t at = pi_of(l31) * (uint32_t)kc.row * (uint32_t)sizeof(T);
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x) kf[x] = row < r1 ? load8(kp, 16 * x + h8, p.k.dim, kvec) : zero_frag<Frag<T>>();
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x) {  // 32 rows of D / 8 pieces, sixty-four at a time
-      const int at = lane + x * 64, r = row0 + at / (D / 8), d = at % (D / 8) * 8;
-      const T *vp = r == place ? vn : vc + (int64_t)r * p.vc.row;
-      vf[x] = r < r1 ? load8(vp, d, p.v.dim, r == place ? p.v.vec : p.vc.vec) : zero_frag<Frag<T>>();
-    }
+    for (int x = 0; x < D / 16; ++x) kf[x] = buffer_load8<T>(kb, at, 16 * x + h8, kc.dim, VEC);
+    vs.load(vc, kv, row0, false, rows);
   };
   if (r0 < r1) fetch(r0);
   for (int row0 = r0; row0 < r1; row0 += 32) {
     f32x16 s = zero16();
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) s = mma(kf[x], qf[x], s);
-#pragma unroll
-    for (int x = 0; x < D / 16; ++x) {
-      const int at = lane + x * 64, r = at / (D / 8), d = at % (D / 8) * 8;
-      const u32x4 *w = (const u32x4 *)&vf[x];
-#pragma unroll
-      for (int y = 0; y < (int)sizeof(T) / 2; ++y)
-        *(u32x4 *)((char *)vt + tile_at<T, D>(r, d + y * (16 / (int)sizeof(T)))) = w[y];
-    }
+    vs.store(vt);
     if (row0 + 32 < r1) fetch(row0 + 32);
     __builtin_amdgcn_wave_barrier();
     float top = -INFINITY;
@@ -268,6 +266,15 @@ struct CacheWriteParams {
 
 constexpr int CW_ROWS = 32;
 
+template <typename T> __device__ inline void copy8(T *to, const T *from, int d, int dim, bool vec) {
+  if (d >= dim) return;
+  if (vec) {
+    *(Frag<T> *)(to + d) = *(const Frag<T> *)(from + d);
+    return;
+  }
+  for (int e = d; e < d + 8 && e < dim; ++e) to[e] = from[e];
+}
+
 // A block takes CW_ROWS places of the cache of one series' slot and looks up which row belongs there.
 template <typename T>
 __global__ __launch_bounds__(256) void window_cache_write_kernel(CacheWriteParams p) {
@@ -297,20 +304,23 @@ __global__ __launch_bounds__(256) void window_cache_write_kernel(CacheWriteParam
         if (t < p.sinks) continue;
       }
       if (t >= m) continue;
-      if (d < p.k.dim) store8(kc + (int64_t)place * p.kc.row, d, p.k.dim, p.kc.vec, load8(kr + (a + t) * p.k.row, d, p.k.dim, p.k.vec));
-      if (d < p.v.dim) store8(vc + (int64_t)place * p.vc.row, d, p.v.dim, p.vc.vec, load8(vr + (a + t) * p.v.row, d, p.v.dim, p.v.vec));
+      copy8(kc + (int64_t)place * p.kc.row, kr + (a + t) * p.k.row, d, p.k.dim, p.k.vec && p.kc.vec);
+      copy8(vc + (int64_t)place * p.vc.row, vr + (a + t) * p.v.row, d, p.v.dim, p.v.vec && p.vc.vec);
     }
   }
 }
 
 // ---- host ----------------------------------------------------------------------------------------
 
-static Rows cache_rows(const tmp_cache &c, int dim, int bytes) {
+static bool cache_rows(const tmp_cache &c, int dim, int bytes, Rows *o) {
   const tmp_rows r = {c.p, c.row_stride, c.head_stride};
-  Rows o = rows_of(r, dim, bytes);
-  if (c.slot_stride % (16 / bytes)) o.vec = 0;
-  return o;
+  const bool ok = rows_of(r, 2, dim, bytes, o);
+  if (c.slot_stride % (16 / bytes)) o->vec = 0;
+  return ok;
 }
+#define TMP_CACHE(what, ref, dim, bytes, to)                                                                   \
+  TMP_REQUIRE(cache_rows(ref, dim, bytes, to), TMP_EUNSUPPORTED,                                               \
+              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements", what)
 
 static int step_check_common(int64_t n, int32_t n_slots, const int32_t *slots, int type, int heads, int dk, int dv,
                              const char *what) {
@@ -346,12 +356,12 @@ static void window_step_split(const tmp_window_attention_step_args *a, int *spli
   *splits = (int)((cap + rows - 1) / rows);
 }
 
-template <typename T, int D> static void window_step(const WindowStepParams &p, hipStream_t st) {
+template <typename T, int D, bool VEC> static void window_step(const WindowStepParams &p, hipStream_t st) {
   const int group = p.heads / p.kv_heads;
   const int units = p.n * p.kv_heads * ((group + 31) / 32) * p.splits;
   {
     ProfScope ps("window_step_kernel", st);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_step_kernel<T, D>), dim3((units + 3) / 4), dim3(256), 4 * 32 * D * sizeof(T), st,
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_step_kernel<T, D, VEC>), dim3((units + 3) / 4), dim3(256), 4 * 32 * D * sizeof(T), st,
                        p, units);
   }
   ProfScope ps("window_join_kernel", st);
@@ -372,8 +382,10 @@ extern "C" int tmp_decay_attention_step(const tmp_decay_attention_step_args *a, 
   const int b = a->type == TMP_F32 ? 4 : 2;
   DecayStepParams p;
   memset(&p, 0, sizeof(p));
-  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b);
-  p.v = rows_of(a->v, a->dim_v, b); p.out = rows_of(a->out, a->dim_v, b);
+  TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p.q);
+  TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p.k);
+  TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p.v);
+  TMP_ROWS(what, a->out, a->n, a->dim_v, b, &p.out);
   p.log_decay = a->log_decay; p.state = a->state; p.slots = a->slots;
   p.n = (int32_t)a->n; p.n_slots = a->n_slots; p.heads = a->heads; p.scale = a->scale;
   const bool vec = ((uintptr_t)a->state & 15) == 0 && a->dim_v % 4 == 0;
@@ -412,9 +424,12 @@ extern "C" int tmp_window_attention_step(const tmp_window_attention_step_args *a
   const int b = a->type == TMP_F32 ? 4 : 2;
   WindowStepParams p;
   memset(&p, 0, sizeof(p));
-  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b);
-  p.v = rows_of(a->v, a->dim_v, b); p.out = rows_of(a->out, a->dim_v, b);
-  p.kc = cache_rows(a->k_cache, a->dim_k, b); p.vc = cache_rows(a->v_cache, a->dim_v, b);
+  TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p.q);
+  TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p.k);
+  TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p.v);
+  TMP_ROWS(what, a->out, a->n, a->dim_v, b, &p.out);
+  TMP_CACHE(what, a->k_cache, a->dim_k, b, &p.kc);
+  TMP_CACHE(what, a->v_cache, a->dim_v, b, &p.vc);
   p.kc_slot = a->k_cache.slot_stride; p.vc_slot = a->v_cache.slot_stride;
   p.length = a->length; p.slots = a->slots; p.part = (float *)workspace;
   p.n = (int32_t)a->n; p.n_slots = a->n_slots; p.heads = a->heads; p.kv_heads = a->kv_heads;
@@ -424,15 +439,7 @@ extern "C" int tmp_window_attention_step(const tmp_window_attention_step_args *a
   TMP_REQUIRE(units < (1ll << 31) - 8, TMP_EUNSUPPORTED, "%s: too many rows x heads", what);
   hipStream_t st = (hipStream_t)stream;
   const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
-  if (a->type == TMP_F32) {
-    if (d == 32) window_step<float, 32>(p, st);
-    else if (d == 64) window_step<float, 64>(p, st);
-    else window_step<float, 128>(p, st);
-  } else {
-    if (d == 32) window_step<__bf16, 32>(p, st);
-    else if (d == 64) window_step<__bf16, 64>(p, st);
-    else window_step<__bf16, 128>(p, st);
-  }
+  TMP_BY_FORM(window_step, a->type, d, p.kc.vec && p.vc.vec, p, st);
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
 }
@@ -453,8 +460,10 @@ extern "C" int tmp_window_cache_write(const tmp_window_cache_write_args *a, void
   CacheWriteParams p;
   memset(&p, 0, sizeof(p));
   p.s.offsets = a->offsets; p.s.n_series = a->n_series; p.s.n = (int32_t)a->n;
-  p.k = rows_of(a->k, a->dim_k, b); p.v = rows_of(a->v, a->dim_v, b);
-  p.kc = cache_rows(a->k_cache, a->dim_k, b); p.vc = cache_rows(a->v_cache, a->dim_v, b);
+  TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p.k);
+  TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p.v);
+  TMP_CACHE(what, a->k_cache, a->dim_k, b, &p.kc);
+  TMP_CACHE(what, a->v_cache, a->dim_v, b, &p.vc);
   p.kc_slot = a->k_cache.slot_stride; p.vc_slot = a->v_cache.slot_stride;
   p.length = a->length; p.slots = a->slots; p.n_slots = a->n_slots; p.kv_heads = a->kv_heads;
   p.window = a->window; p.sinks = a->sinks;

@@ -66,63 +66,76 @@ __device__ inline Span walk_span(const DecayParams &p, int pos) {
 
 // A wave's state: all of dk, 32 of dv.  Tile t's register x is dk = 32 t + 16 (x / 8) + 8 (lane / 32) + x % 8,
 // the lane is dv = strip + pi(lane % 32).
+__device__ inline uint32_t state_at(int lane, int t, int x, int kd, int vd, bool transposed) {
+  const int dk = 32 * t + 16 * (x >> 3) + (lane >> 5) * 8 + (x & 7), dv = (threadIdx.x >> 6) * 32 + pi_of(lane & 31);
+  return dk < kd && dv < vd ? (transposed ? dv * kd + dk : dk * vd + dv) * 4 : kOutside;
+}
 template <int NT> __device__ inline void state_load(f32x16 (&st)[NT], const float *p, int kd, int vd, bool transposed, float by) {
-  const int h8 = (lane_id() >> 5) * 8, dv = (threadIdx.x >> 6) * 32 + pi_of(lane_id() & 31);
-  asm volatile("" : "+v"(vd), "+v"(kd));  // (keeps the addresses from being held in registers over the walk)
+  const Buffer b = buffer_of(p, kd * vd * 4);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));  // (keeps the offsets from being held in registers over the walk)
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const int dk = 32 * t + 16 * (x >> 3) + h8 + (x & 7);
-      st[t][x] = dk < kd && dv < vd ? p[transposed ? dv * kd + dk : dk * vd + dv] * by : 0.f;
-    }
+    for (int x = 0; x < 16; ++x)
+      st[t][x] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, state_at(lane, t, x, kd, vd, transposed), 0, 0)) * by;
+  }
 }
 template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], float *p, int kd, int vd, bool transposed, float by) {
-  const int h8 = (lane_id() >> 5) * 8, dv = (threadIdx.x >> 6) * 32 + pi_of(lane_id() & 31);
-  asm volatile("" : "+v"(vd), "+v"(kd));  // (keeps the addresses from being held in registers over the walk)
+  const Buffer b = buffer_of(p, kd * vd * 4);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int t = 0; t < NT; ++t) {
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const int dk = 32 * t + 16 * (x >> 3) + h8 + (x & 7);
-      if (dk < kd && dv < vd) p[transposed ? dv * kd + dk : dk * vd + dv] = st[t][x] * by;
-    }
+    for (int x = 0; x < 16; ++x)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, st[t][x] * by), b, state_at(lane, t, x, kd, vd, transposed), 0, 0);
+  }
 }
 
-// X <- lambda^len X + K^T diag(lambda^{len-1-s+post}) V.  The weighted values do not fit bfloat16; they
-// enter as the sum of two such numbers (2^-18 of a term), three where the state itself is returned (2^-27).
-template <int D> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int b, const float *w, bf16x8 v, bool exact) {
-  bf16x8 hi, lo, rest;
+// X <- X + K^T diag(w) V for sixteen rows.  The weighted values do not fit bfloat16; they enter as the sum
+// of two such numbers (2^-18 of a term), three where the state itself is returned (2^-27).
+template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int k0, const float *w, bf16x8 v) {
+  bf16x8 hi, lo;
+  f32x8 x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = (float)v[e] * w[e];
-    hi[e] = (__bf16)x;
-    const float y = x - (float)hi[e];
-    lo[e] = (__bf16)y;
-    rest[e] = (__bf16)(y - (float)lo[e]);
+  for (int e = 0; e < 8; ++e) x[e] = (float)v[e] * w[e];
+  hi = __builtin_convertvector(x, bf16x8);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] -= (float)hi[e];
+  lo = __builtin_convertvector(x, bf16x8);
+  bf16x8 rest;
+  if (EXACT) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= (float)lo[e];
+    rest = __builtin_convertvector(x, bf16x8);
   }
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) {
-    const bf16x8 kf = col_frag<D>(kt, 16 * b, 32 * t);
+    const bf16x8 kf = col_frag<D>(kt, k0, 32 * t);
     st[t] = mma(kf, hi, st[t]);
     st[t] = mma(kf, lo, st[t]);
-    if (exact) st[t] = mma(kf, rest, st[t]);
+    if (EXACT) st[t] = mma(kf, rest, st[t]);
   }
 }
-template <int D> __device__ inline void state_add(f32x16 (&st)[D / 32], const float *kt, int b, const float *w, f32x8 v, bool) {
+template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const float *kt, int k0, const float *w, f32x8 v) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] *= w[e];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, 16 * b, 32 * t), v, st[t]);
+  for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, k0, 32 * t), v, st[t]);
 }
 
 // OUT: walks a section and writes its rows.  Otherwise: walks the rows of the section that belong to the
 // series which goes on behind it, and leaves the state that they make in carry[section + 1].
-template <typename T, int D, bool OUT>
-__global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
-  constexpr int NT = D / 32, THREADS = D * 2;
+//
+// A wave owns 32 columns of the values and that strip of the state, in registers; the queries', keys' and
+// values' tiles of 64 rows are shared, the next ones on their way meanwhile.  Rows are worked on in parts of
+// SUB, whose decays are the same for every part (held in registers) but a series' last one.
+template <typename T, int D, bool VEC, bool OUT, bool EXACT>
+__global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2) void decay_walk_kernel(DecayParams p) {
+  constexpr int NT = D / 32, THREADS = D * 2, SUB = 32;
   const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
-  const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = (threadIdx.x >> 6) * 32;
+  const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
   const int kd = p.k.dim, vd = p.v.dim;
   const int64_t per_state = (int64_t)kd * vd;
   const int sec0 = sec * p.section, sec1 = sec0 + p.section < p.s.n ? sec0 + p.section : p.s.n;
@@ -143,27 +156,27 @@ __global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   const float ld = p.log_decay[head] * kLog2e;
   const int post = p.reverse ? 1 : 0;
-  const T *qp = head_of<T>(p.q, head), *kp = head_of<T>(p.k, head), *vp = head_of<T>(p.v, head);
-  float wd[16], wo[16];  // lambda^{i-j} of a 32 x 32 piece on the diagonal, and of the one below it
+  float wd[16];  // scale lambda^{i-j} of a part's rows i and j <= i
   if (OUT)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       const int j = 16 * (x >> 3) + h8 + (x & 7);
-      wd[x] = j <= l31 ? power(ld, l31 - j) : 0.f;
-      wo[x] = power(ld, 32 + l31 - j);
+      wd[x] = j <= l31 ? p.scale * power(ld, l31 - j) : 0.f;
     }
-  const float into[2] = {power(ld, l31 + 1 - post), power(ld, l31 + 33 - post)};
+  const float into = p.scale * power(ld, l31 + 1 - post), fade_all = power(ld, SUB);
+  float w_all[SUB / 2];  // lambda^{SUB-1-s+post}
+#pragma unroll
+  for (int e = 0; e < SUB / 2; ++e) w_all[e] = power(ld, SUB - 1 - (16 * (e >> 3) + h8 + (e & 7)) + post);
   f32x16 st[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) st[t] = zero16();
-  bool has = false, fresh = true;
-  Staged<T, D, DA_PIECE, THREADS> qs, ks, vs;
+  bool fresh = true;
+  Staged<T, D, DA_PIECE, THREADS, VEC, true> qs, ks, vs;
   auto fetch = [&](int at, int len) {
     const int64_t first = p.reverse ? (int64_t)p.s.n - 1 - at : at;
-    const int step = p.reverse ? -1 : 1;
-    ks.load(kp, p.k.row, kd, p.k.vec, first, step, len);
-    vs.load(vp, p.v.row, vd, p.v.vec, first, step, len);
-    if (OUT) qs.load(qp, p.q.row, p.q.dim, p.q.vec, first, step, len);
+    ks.load(p.k, head, first, p.reverse, len);
+    vs.load(p.v, head, first, p.reverse, len);
+    if (OUT) qs.load(p.q, head, first, p.reverse, len);
   };
   auto length = [&](int at, const Span &s) {
     int e = s.end < sec1 ? s.end : sec1;
@@ -174,12 +187,28 @@ __global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
   while (true) {
     __syncthreads();
     ks.store(kt);
-    if (vs.store(vt)) flag[turn] = 1;
-    if (OUT) qs.store(qt);
+    vs.store(vt);
+    if (OUT) {
+      qs.store(qt);
+      if (vs.dirty()) flag[turn] = 1;
+    }
     if (threadIdx.x == 0) flag[turn ^ 1] = 0;
     __syncthreads();
     const bool dirty = OUT && flag[turn];
     turn ^= 1;
+    int bad[2] = {DA_PIECE, DA_PIECE};  // of the lane's column, in either half: the first row that is not finite
+    if (__builtin_expect(dirty, 0)) {
+#pragma unroll 1
+      for (int j = 0; j < DA_PIECE; ++j) {
+        const bool on = !finite(tile_elem<T, D>(vt, j, strip + pi_of(l31)));
+        if (j < 32) bad[0] = on && j < bad[0] ? j : bad[0];
+        else bad[1] = on && j - 32 < bad[1] ? j - 32 : bad[1];
+      }
+      __syncthreads();
+      vs.clean();  // (a zero weight would not keep such values out of the rows before them)
+      vs.store(vt);
+      __syncthreads();
+    }
     const int next = pos + len;
     Span nsp = sp;
     int nlen = 0;
@@ -188,12 +217,12 @@ __global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
       nlen = length(next, nsp);
       fetch(next, nsp.index < 0 ? 0 : nlen);
     }
+    const bool ends = next >= sp.end;
     if (fresh) {
       const float *from = sp.index < 0 ? nullptr
                           : sp.start < pos ? (OUT ? p.carry + ((int64_t)sec * p.heads + head) * per_state : nullptr)
                           : p.state_in ? p.state_in + ((int64_t)sp.index * p.heads + head) * per_state : nullptr;
-      has = from != nullptr;
-      if (has) {
+      if (from) {
         const bool own = sp.start < pos;  // a carry lies as this walk left it
         state_load(st, from, kd, vd, !own && p.transposed, own ? 1.f : p.in_by);
       } else {
@@ -201,100 +230,70 @@ __global__ __launch_bounds__(D * 2, 1) void decay_walk_kernel(DecayParams p) {
         for (int t = 0; t < NT; ++t) st[t] = zero16();
       }
     }
-    if (OUT) {
-      f32x16 acc[2] = {zero16(), zero16()};
-      if (has) {
+#pragma unroll 1
+    for (int r0 = 0; r0 < len; r0 += SUB) {
+      const int rows = len - r0 < SUB ? len - r0 : SUB;
+      if (OUT) {
+        f32x16 acc = zero16(), s = zero16();
 #pragma unroll
         for (int b = 0; b < D / 16; ++b) {
-          const Frag<T> sf = operand<T>(st[b >> 1], b & 1);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) acc[i] = mma(sf, row_frag<D>(qt, i * 32 + l31, 16 * b + h8), acc[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) acc[i][x] *= into[i];
-      }
-      if (sp.index >= 0) {
-        f32x16 s00 = zero16(), s01 = zero16(), s11 = zero16();  // [key half][row half]
-#pragma unroll
-        for (int b = 0; b < D / 16; ++b) {
-          const Frag<T> k0 = row_frag<D>(kt, pi_of(l31), 16 * b + h8), q0 = row_frag<D>(qt, l31, 16 * b + h8);
-          s00 = mma(k0, q0, s00);
-          if (len > 32) {
-            const Frag<T> k1 = row_frag<D>(kt, 32 + pi_of(l31), 16 * b + h8), q1 = row_frag<D>(qt, 32 + l31, 16 * b + h8);
-            s01 = mma(k0, q1, s01);
-            s11 = mma(k1, q1, s11);
-          }
+          const Frag<T> qf = row_frag<D>(qt, r0 + l31, 16 * b + h8);
+          s = mma(row_frag<D>(kt, r0 + pi_of(l31), 16 * b + h8), qf, s);
+          acc = mma(operand<T>(st[b >> 1], b & 1), qf, acc);
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const bool on = 16 * (x >> 3) + h8 + (x & 7) <= l31;
-          s00[x] = on ? s00[x] * wd[x] : 0.f;
-          s11[x] = on ? s11[x] * wd[x] : 0.f;
-          s01[x] *= wo[x];
+          acc[x] *= into;
+          s[x] = 16 * (x >> 3) + h8 + (x & 7) <= l31 ? s[x] * wd[x] : 0.f;
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          Frag<T> v0 = col_frag<D>(vt, 16 * b, strip);
-          if (dirty) v0 = cleaned(v0);
-          acc[0] = mma(v0, operand<T>(s00, b), acc[0]);
-          if (len > 32) {
-            Frag<T> v1 = col_frag<D>(vt, 32 + 16 * b, strip);
-            if (dirty) v1 = cleaned(v1);
-            acc[1] = mma(v0, operand<T>(s01, b), acc[1]);
-            acc[1] = mma(v1, operand<T>(s11, b), acc[1]);
+        for (int b = 0; b < 2; ++b) acc = mma(col_frag<D>(vt, r0 + 16 * b, strip), operand<T>(s, b), acc);
+        if (__builtin_expect(dirty, 0)) {  // they reach the rows at and behind their own, as NaN
+          const int first = r0 ? bad[1] : bad[0];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const int at = __shfl(first, pi_of(16 * (x >> 3) + h8 + (x & 7)));
+            acc[x] = at <= l31 ? __uint_as_float(0x7fc00000u) : acc[x];
           }
         }
-        if (dirty)  // values that are not finite reach the rows at and behind their own, as NaN
-#pragma unroll 1
-          for (int j = 0; j < len; ++j) {
-            int at = j;
-            asm volatile("" : "+v"(at));  // keeps the addresses below out of the registers of the main path
+        const int r = pos + r0;
+        const Run o = rows_buffer<T>(p.out, head, p.reverse ? (int64_t)p.s.n - r - rows : r, rows);
+        const uint32_t at = (uint32_t)((p.reverse ? rows - 1 - l31 : l31) * (int)p.out.row * (int)sizeof(T));
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const float y = tile_elem<T, D>(vt, at, strip + 16 * (x >> 3) + h8 + (x & 7));
-                if (j <= i * 32 + l31 && !finite(y)) acc[i][x] += y - y;
-                if ((x & 3) == 3) __builtin_amdgcn_sched_barrier(0);
-              }
-          }
+        for (int b = 0; b < 2; ++b) buffer_store8(o, at, strip + 16 * b + h8, p.out.dim, VEC, operand<T>(acc, b));
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = i * 32 + l31;
-        if (r >= len) continue;
-        const int64_t row = p.reverse ? (int64_t)p.s.n - 1 - (pos + r) : pos + r;
-        T *o = (T *)p.out.p + (int64_t)head * p.out.head + row * p.out.row;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[i][x] *= p.scale;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) store8(o, strip + 16 * b + h8, p.out.dim, p.out.vec, operand<T>(acc[i], b));
-      }
-    }
-    const bool ends = next >= sp.end;
-    if (sp.index >= 0 && (!ends || p.state_out)) {
-      const float fade = power(ld, len);
+      if (sp.index < 0 || (ends && r0 + SUB >= len && !p.state_out)) continue;  // no state, or nobody reads it
+      const float fade = rows == SUB ? fade_all : power(ld, rows);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int x = 0; x < 16; ++x) st[t][x] *= fade;
+      if (rows == SUB) {
 #pragma unroll
-      for (int b = 0; b < DA_PIECE / 16; ++b) {
-        if (16 * b >= len) break;
-        float w[8];
+        for (int b = 0; b < SUB / 16; ++b)
+          state_add<D, EXACT>(st, kt, r0 + 16 * b, w_all + 8 * b, col_frag<D>(vt, r0 + 16 * b, strip));
+      } else {
+#pragma unroll 1
+        for (int b = 0; 16 * b < rows; ++b) {
+          float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int left = len - 1 - (16 * b + h8 + e);
-          w[e] = left >= 0 ? power(ld, left + post) : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            const int left = rows - 1 - (16 * b + h8 + e);
+            w[e] = left >= 0 ? power(ld, left + post) : 0.f;
+          }
+          state_add<D, EXACT>(st, kt, r0 + 16 * b, w, col_frag<D>(vt, r0 + 16 * b, strip));
         }
-        state_add<D>(st, kt, b, w, col_frag<D>(vt, 16 * b, strip), p.state_out != nullptr);
       }
-      has = true;
-      if (OUT && ends)
-        state_store(st, p.state_out + ((int64_t)sp.index * p.heads + head) * per_state, kd, vd, p.transposed, p.out_by);
+      if (__builtin_expect(dirty, 0)) {
+        const float x = (r0 ? bad[1] : bad[0]) < DA_PIECE ? __uint_as_float(0x7fc00000u) : 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int y = 0; y < 16; ++y) st[t][y] += x;
+      }
     }
+    if (OUT && ends && sp.index >= 0 && p.state_out)
+      state_store(st, p.state_out + ((int64_t)sp.index * p.heads + head) * per_state, kd, vd, p.transposed, p.out_by);
     fresh = ends;
     if (next >= sec1) break;
     pos = next;
@@ -389,27 +388,30 @@ static int decay_check(const tmp_decay_attention_args *a, const char *what, bool
   return TMP_OK;
 }
 
-template <typename T, int D> static int decay_walk(const DecayParams &p, hipStream_t st) {
+template <typename T, int D, bool VEC, bool EXACT> static void decay_walk(const DecayParams &p, hipStream_t st) {
   const int threads = D * 2, piece = DA_PIECE * D * (int)sizeof(T);
   if (p.sections > 1) {
     {
       ProfScope ps("decay_walk_kernel(states)", st);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, false>), dim3((p.sections - 1) * p.heads), dim3(threads),
-                         2 * piece, st, p);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, VEC, false, EXACT>), dim3((p.sections - 1) * p.heads),
+                         dim3(threads), 2 * piece, st, p);
     }
     const int64_t per_head = (int64_t)p.k.dim * p.v.dim;
     TMP_LAUNCH(decay_scan_kernel, dim3((unsigned)((per_head + 255) / 256 * p.heads)), dim3(256), st, p, per_head);
   }
   ProfScope ps("decay_walk_kernel", st);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, true>), dim3(p.sections * p.heads), dim3(threads), 3 * piece, st, p);
-  return TMP_OK;
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, VEC, true, EXACT>), dim3(p.sections * p.heads), dim3(threads),
+                     3 * piece, st, p);
+}
+template <typename T, int D, bool VEC> static void decay_walk_form(const DecayParams &p, hipStream_t st) {
+  if (sizeof(T) == 2 && p.state_out) decay_walk<T, D, VEC, sizeof(T) == 2>(p, st);
+  else decay_walk<T, D, VEC, false>(p, st);
 }
 
-static int decay_run(const DecayParams &p, int type, hipStream_t st) {
+static void decay_run(const DecayParams &p, int type, hipStream_t st) {
   const int d = padded_dim(p.k.dim > p.v.dim ? p.k.dim : p.v.dim);
-  if (type == TMP_F32)
-    return d == 32 ? decay_walk<float, 32>(p, st) : d == 64 ? decay_walk<float, 64>(p, st) : decay_walk<float, 128>(p, st);
-  return d == 32 ? decay_walk<__bf16, 32>(p, st) : d == 64 ? decay_walk<__bf16, 64>(p, st) : decay_walk<__bf16, 128>(p, st);
+  const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec;
+  TMP_BY_FORM(decay_walk_form, type, d, vec, p, st);
 }
 
 static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d) {
@@ -450,10 +452,15 @@ extern "C" int tmp_decay_attention(const tmp_decay_attention_args *a, void *work
   hipStream_t st = (hipStream_t)stream;
   const int b = a->type == TMP_F32 ? 4 : 2;
   DecayParams p = decay_params(a, d);
-  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b);
-  p.v = rows_of(a->v, a->dim_v, b); p.out = rows_of(a->out, a->dim_v, b);
+  const char *what = "tmp_decay_attention";
+  if (a->n > 0) {
+    TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p.q);
+    TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p.k);
+    TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p.v);
+    TMP_ROWS(what, a->out, a->n, a->dim_v, b, &p.out);
+  }
   p.state_in = a->state_in; p.state_out = a->state_out;
-  if (a->n > 0) TMP_TRY(decay_run(p, a->type, st));
+  if (a->n > 0) decay_run(p, a->type, st);
   TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
@@ -468,21 +475,30 @@ extern "C" int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void 
   TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_decay_attention_grad: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   const int b = a->type == TMP_F32 ? 4 : 2;
-  const Rows q = rows_of(a->q, a->dim_k, b), k = rows_of(a->k, a->dim_k, b), v = rows_of(a->v, a->dim_v, b);
-  const Rows o = rows_of(a->dout, a->dim_v, b);
+  const char *what = "tmp_decay_attention_grad";
+  Rows q = {}, k = {}, v = {}, o = {}, dq = {}, dk = {}, dv = {};
+  if (a->n > 0) {
+    TMP_ROWS(what, a->q, a->n, a->dim_k, b, &q);
+    TMP_ROWS(what, a->k, a->n, a->dim_k, b, &k);
+    TMP_ROWS(what, a->v, a->n, a->dim_v, b, &v);
+    TMP_ROWS(what, a->dout, a->n, a->dim_v, b, &o);
+    TMP_ROWS(what, a->dq, a->n, a->dim_k, b, &dq);
+    TMP_ROWS(what, a->dk, a->n, a->dim_k, b, &dk);
+    TMP_ROWS(what, a->dv, a->n, a->dim_v, b, &dv);
+  }
   DecayParams p = decay_params(a, d);
   if (a->n > 0) {
-    p.q = o; p.k = v; p.v = k; p.out = rows_of(a->dq, a->dim_k, b);
+    p.q = o; p.k = v; p.v = k; p.out = dq;
     p.state_in = a->state_in; p.transposed = 1;
-    TMP_TRY(decay_run(p, a->type, st));
+    decay_run(p, a->type, st);
   }
   p.reverse = 1; p.state_in = a->dstate_out; p.in_by = 1.f / a->scale; p.out_by = a->scale;
   if (a->n > 0) {
-    p.q = v; p.k = o; p.v = q; p.out = rows_of(a->dk, a->dim_k, b);
-    TMP_TRY(decay_run(p, a->type, st));
-    p.q = k; p.k = q; p.v = o; p.out = rows_of(a->dv, a->dim_v, b);
+    p.q = v; p.k = o; p.v = q; p.out = dk;
+    decay_run(p, a->type, st);
+    p.q = k; p.k = q; p.v = o; p.out = dv;
     p.transposed = 0; p.state_out = a->dstate_in;
-    TMP_TRY(decay_run(p, a->type, st));
+    decay_run(p, a->type, st);
   }
   p.state_out = a->dstate_in;
   TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));

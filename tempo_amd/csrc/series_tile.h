@@ -81,18 +81,21 @@ template <> __device__ inline f32x8 operand<float>(const f32x16 &c, int b) {
 // ---- values that are not finite -------------------------------------------------------------
 // A masked position must not reach a result, and 0 * NaN would.  Tiles are looked at as they are
 // staged; a tile that holds such a value (rare) has its operands cleaned and the visible ones added.
-__device__ inline uint32_t not_finite(u32x4 v, __bf16) {  // nonzero if a half has all exponent bits set
-  uint32_t bad = 0;
+// The largest magnitude bits seen so far, two halves (bfloat16) or a word (float) at a time.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t magnitude(uint32_t most, u32x4 v, __bf16) {
+  u16x2 m = __builtin_bit_cast(u16x2, most);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= ((v[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-  return bad;
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+  return __builtin_bit_cast(uint32_t, m);
 }
-__device__ inline uint32_t not_finite(u32x4 v, float) {
-  uint32_t bad = 0;
+__device__ inline uint32_t magnitude(uint32_t most, u32x4 v, float) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= ((v[i] & 0x7f800000u) + 0x00800000u) & 0x80000000u;
-  return bad;
+  for (int i = 0; i < 4; ++i) most = max(most, v[i] & 0x7fffffffu);
+  return most;
 }
+__device__ inline bool not_finite(uint32_t most, __bf16) { return (most & 0x7f80u) == 0x7f80u || (most >> 16) >= 0x7f80u; }
+__device__ inline bool not_finite(uint32_t most, float) { return most >= 0x7f800000u; }
 __device__ inline bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 template <typename F> __device__ inline F cleaned(F f) {
 #pragma unroll
@@ -102,8 +105,13 @@ template <typename F> __device__ inline F cleaned(F f) {
 }
 
 // ---- rows in memory --------------------------------------------------------------------------
-// Rows of one head: element d of row r at p + r * stride + d, d < dim.  vec: 16-byte loads are allowed
-// (pointer and strides multiples of 16 bytes, dim a multiple of eight elements), decided by the host.
+// Rows of one head: element d of row r at p + r * row + d, d < dim, dim <= row < 2^22 (checked by the
+// host), so that a hundred rows are within reach of 32-bit byte offsets.  vec: 16-byte accesses are allowed
+// (pointer and strides multiples of 16 bytes, dim a multiple of eight elements), decided by the host;
+// kernels come in two forms, VEC for calls whose every array allows them.
+//
+// A run of rows is accessed through a buffer descriptor that ends behind its last row: what lies outside
+// reads as zero and is not written, so that odd lengths and head sizes cost no branch.
 struct Rows {
   void *p;
   int64_t row, head;  // strides in elements
@@ -114,50 +122,88 @@ template <typename T> __device__ inline const T *head_of(const Rows &r, int head
   return (const T *)r.p + (int64_t)head * r.head;
 }
 
-// Eight elements from d on of the row at `p`, zeros beyond dim.
-__device__ inline bf16x8 load8(const __bf16 *p, int d, int dim, bool vec) {
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ inline Buffer buffer_of(const void *p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, bytes, 0x00020000);
+}
+// Rows [first, first + count) of a head.  The descriptor's address has to be a multiple of four bytes: `lead` is
+// how far the first row lies behind it.
+struct Run {
+  Buffer b;
+  uint32_t lead;
+};
+template <typename T> __device__ inline Run rows_buffer(const Rows &r, int head, int64_t first, int count) {
+  // (the same for all lanes of a wave: said to the compiler, which would loop over the lanes' values otherwise)
+  const uint64_t at = (uint64_t)(head_of<T>(r, head) + first * r.row);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+  const uint32_t bytes = (uint32_t)count * (uint32_t)r.row * (uint32_t)sizeof(T), lead = lo & 3;
+  Run run;
+  run.b = buffer_of((void *)(((uint64_t)hi << 32) | (lo & ~3u)), __builtin_amdgcn_readfirstlane(bytes) + lead);
+  run.lead = lead;
+  return run;
+}
+constexpr uint32_t kOutside = 0xfffffff0u;  // a byte offset behind every buffer's end
+
+// Eight elements from d on of the row that starts `at` bytes into the buffer, zeros beyond dim.
+template <typename T> __device__ inline Frag<T> buffer_load8(Run u, uint32_t at, int d, int dim, bool vec);
+template <> __device__ inline bf16x8 buffer_load8<__bf16>(Run u, uint32_t at, int d, int dim, bool vec) {
+  const Buffer b = u.b;
+  if (vec) return __builtin_bit_cast(bf16x8, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, d < dim ? at + d * 2 : kOutside, 0, 0));
   bf16x8 f;
-  if (vec && d < dim) return *(const bf16x8 *)(p + d);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = d + e < dim ? p[d + e] : (__bf16)0.f;
+  for (int e = 0; e < 8; ++e)
+    f[e] = __builtin_bit_cast(__bf16, __builtin_amdgcn_raw_buffer_load_b16(b, d + e < dim ? u.lead + at + (d + e) * 2 : kOutside, 0, 0));
   return f;
 }
-__device__ inline f32x8 load8(const float *p, int d, int dim, bool vec) {
+template <> __device__ inline f32x8 buffer_load8<float>(Run u, uint32_t at, int d, int dim, bool vec) {
+  const Buffer b = u.b;
   f32x8 f;
-  if (vec && d < dim) {
-    const f32x4 a = *(const f32x4 *)(p + d), b = *(const f32x4 *)(p + d + 4);
+  if (vec) {
+    const uint32_t o = d < dim ? at + d * 4 : kOutside;
+    const f32x4 x = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, o, 0, 0));
+    const f32x4 y = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, d < dim ? o + 16 : kOutside, 0, 0));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { f[e] = a[e]; f[e + 4] = b[e]; }
+    for (int e = 0; e < 4; ++e) { f[e] = x[e]; f[e + 4] = y[e]; }
     return f;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = d + e < dim ? p[d + e] : 0.f;
+  for (int e = 0; e < 8; ++e)
+    f[e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, d + e < dim ? at + (d + e) * 4 : kOutside, 0, 0));
   return f;
+}
+__device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, bf16x8 f) {
+  const Buffer b = u.b;
+  if (vec) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), b, d < dim ? at + d * 2 : kOutside, 0, 0);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const __bf16 x = f[e];
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x), b, d + e < dim ? u.lead + at + (d + e) * 2 : kOutside, 0, 0);
+  }
+}
+__device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, f32x8 f) {
+  const Buffer b = u.b;
+  if (vec) {
+    f32x4 x, y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x[e] = f[e]; y[e] = f[e + 4]; }
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), b, d < dim ? at + d * 4 : kOutside, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), b, d < dim ? at + d * 4 + 16 : kOutside, 0, 0);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = f[e];
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), b, d + e < dim ? at + (d + e) * 4 : kOutside, 0, 0);
+  }
 }
 template <typename F> __device__ inline F zero_frag() {
   F f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = 0;
   return f;
-}
-__device__ inline void store8(__bf16 *p, int d, int dim, bool vec, bf16x8 f) {
-  if (vec && d < dim) { *(bf16x8 *)(p + d) = f; return; }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (d + e < dim) p[d + e] = f[e];
-}
-__device__ inline void store8(float *p, int d, int dim, bool vec, f32x8 f) {
-  if (vec && d < dim) {
-    f32x4 a, b;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { a[e] = f[e]; b[e] = f[e + 4]; }
-    *(f32x4 *)(p + d) = a;
-    *(f32x4 *)(p + d + 4) = b;
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (d + e < dim) p[d + e] = f[e];
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------
@@ -223,32 +269,50 @@ template <typename T, int D> __device__ inline float tile_elem(const T *t, int r
 
 // A tile on its way from memory to LDS, by THREADS consecutive threads of the block: loads are issued by load(), waited for and written by store(),
 // so that a tile travels while the one before it is worked on.
-template <typename T, int D, int ROWS, int THREADS> struct Staged {
+template <typename T, int D, int ROWS, int THREADS, bool VEC, bool FRESH = false> struct Staged {
   static constexpr int kPerRow = D / 8;
-  static constexpr int kCount = (ROWS * kPerRow + THREADS - 1) / THREADS;
+  static constexpr int kCount = ROWS * kPerRow / THREADS;
+  static_assert(ROWS * kPerRow % THREADS == 0 && THREADS % kPerRow == 0, "whole pieces");
+  static constexpr int kStep = THREADS / kPerRow;  // rows from one of a thread's pieces to its next
   Frag<T> f[kCount];
-  // rows first + step * r for r in [0, count) are read, the others become zeros
-  __device__ inline void load(const T *p, int64_t row_stride, int dim, bool vec, int64_t first, int step, int count) {
+  // rows first + r, or with `back` first - r, for r in [0, count) are read, the others become zeros
+  __device__ inline void load(const Rows &rows, int head, int64_t first, bool back, int count) {
+    const int tid = threadIdx.x % THREADS, r0 = tid / kPerRow, d = (tid % kPerRow) * 8;
+    const Run b = rows_buffer<T>(rows, head, back ? first - (count - 1) : first, count);
+    const int row = (int)rows.row * (int)sizeof(T);
+    // (backwards, rows from `count` on lie before the buffer: offsets below zero, which are outside too)
+    int at = back ? (count - 1 - r0) * row : r0 * row;
+    const int step = (back ? -kStep : kStep) * row;
+    if (FRESH) asm volatile("" : "+v"(at));  // (the pieces' offsets are worked out anew each time: cheaper than registers)
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const int at = threadIdx.x % THREADS + i * THREADS, r = at / kPerRow, d = (at % kPerRow) * 8;
-      f[i] = r < count && d < dim ? load8(p + (first + (int64_t)step * r) * row_stride, d, dim, vec) : zero_frag<Frag<T>>();
+      int from = at + i * step;
+      if (!VEC) asm volatile("" : "+v"(from));  // (offsets of single elements are not worth registers)
+      f[i] = buffer_load8<T>(b, from, d, VEC || r0 + i * kStep < count ? rows.dim : 0, VEC);
     }
   }
-  __device__ inline uint32_t store(T *t) const {  // whether it holds a value that is not finite
-    uint32_t bad = 0;
+  __device__ inline void store(T *t) const {
+    const int tid = threadIdx.x % THREADS, r0 = tid / kPerRow, d = (tid % kPerRow) * 8;
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      const int at = threadIdx.x % THREADS + i * THREADS, r = at / kPerRow, d = (at % kPerRow) * 8;
-      if (ROWS * kPerRow % THREADS && r >= ROWS) continue;
+      const int r = r0 + i * kStep;
       const u32x4 *w = (const u32x4 *)&f[i];
 #pragma unroll
-      for (int c = 0; c < (int)sizeof(T) / 2; ++c) {
-        bad |= not_finite(w[c], T());
+      for (int c = 0; c < (int)sizeof(T) / 2; ++c)
         *(u32x4 *)((char *)t + tile_at<T, D>(r, d + c * (16 / (int)sizeof(T)))) = w[c];
-      }
     }
-    return bad;
+  }
+  __device__ inline void clean() {  // zeros in place of what is not finite
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) f[i] = cleaned(f[i]);
+  }
+  __device__ inline bool dirty() const {  // whether a value is not finite
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+#pragma unroll
+      for (int c = 0; c < (int)sizeof(T) / 2; ++c) most = magnitude(most, ((const u32x4 *)&f[i])[c], T());
+    return not_finite(most, T());
   }
 };
 
@@ -318,13 +382,35 @@ __device__ inline int item_of_block(int total) {
 inline int grid_of_items(int64_t total) { return (int)((total + 7) / 8 * 8); }
 
 // ---- host side -------------------------------------------------------------------------------
-inline Rows rows_of(const tmp_rows &r, int dim, int bytes) {
-  Rows o;
-  o.p = r.p; o.row = r.row_stride; o.head = r.head_stride; o.dim = dim;
+// Rows of `n`, dim elements each; false: strides that the kernels do not take.
+inline bool rows_of(const tmp_rows &r, int64_t n, int dim, int bytes, Rows *o) {
   const int64_t per = 16 / bytes;
-  o.vec = ((uintptr_t)r.p & 15) == 0 && r.row_stride % per == 0 && r.head_stride % per == 0 && dim % 8 == 0;
-  return o;
+  o->p = r.p; o->row = n > 1 ? r.row_stride : (dim + 7) / 8 * 8; o->head = r.head_stride; o->dim = dim;
+  o->vec = ((uintptr_t)r.p & 15) == 0 && o->row % per == 0 && r.head_stride % per == 0 && dim % 8 == 0;
+  return o->row >= dim && o->row < (1 << 22);
 }
+#define TMP_ROWS(what, ref, n, dim, bytes, to)                                                                 \
+  TMP_REQUIRE(rows_of(ref, n, dim, bytes, to), TMP_EUNSUPPORTED,                                               \
+              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements", what)
+
+// fn<T, D, VEC>(...) for a type, a padded head size and an access width.
+#define TMP_BY_DIM(fn, T, d, VEC, ...)              \
+  do {                                              \
+    if ((d) == 32) fn<T, 32, VEC>(__VA_ARGS__);     \
+    else if ((d) == 64) fn<T, 64, VEC>(__VA_ARGS__); \
+    else fn<T, 128, VEC>(__VA_ARGS__);              \
+  } while (0)
+#define TMP_BY_FORM(fn, type, d, vec, ...)                             \
+  do {                                                                 \
+    if ((type) == TMP_F32) {                                           \
+      if (vec) TMP_BY_DIM(fn, float, d, true, __VA_ARGS__);            \
+      else TMP_BY_DIM(fn, float, d, false, __VA_ARGS__);               \
+    } else {                                                           \
+      if (vec) TMP_BY_DIM(fn, __bf16, d, true, __VA_ARGS__);           \
+      else TMP_BY_DIM(fn, __bf16, d, false, __VA_ARGS__);              \
+    }                                                                  \
+  } while (0)
+
 inline int padded_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 }  // namespace tmp

@@ -31,12 +31,16 @@ struct WindowParams {
   float scale;
 };
 
-struct Seen {  // which rows j a row i sees
-  int window, sinks;
-  __device__ inline bool operator()(int i, int j, int start) const {
-    return j <= i && j >= start && (j > i - window || j < start + sinks);
-  }
+// Which streamed rows a lane's own row sees (or is seen by), as runs of the tile's rows: [lo, hi] of the window and
+// [slo, shi] of the rows that stay visible.
+struct Seen {
+  int lo, hi, slo, shi;
+  __device__ inline Seen from(int x) const { return {lo - x, hi - x, slo - x, shi - x}; }
+  __device__ inline bool operator()(int x) const { return ((x >= lo) & (x <= hi)) | ((x >= slo) & (x <= shi)); }
 };
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+__device__ inline int min_of(int a, int b) { return a < b ? a : b; }
+__device__ inline int max_of(int a, int b) { return a > b ? a : b; }
 
 // What a wave knows of its 32 own rows when they are query rows.
 struct QueryRows {
@@ -53,7 +57,7 @@ __device__ inline QueryRows query_rows(const WindowParams &p, int t0) {
   const int c0 = count_le(p.s, t0, 0, most);
   int c1 = c0;
   if (p.s.offsets && c0 < most && p.s.offsets[c0] < t1) c1 = count_le(p.s, t1 - 1, c0, most);
-  r.i = t0 + (threadIdx.x >> 6) * 32 + (lane_id() & 31);
+  r.i = t0 + wave_id() * 32 + (lane_id() & 31);
   const Span first = span_at(p.s, c0, t0);
   r.first_start = first.start < t0 ? first.start : t0;
   const int w = t0 - p.window + 1;
@@ -63,7 +67,7 @@ __device__ inline QueryRows query_rows(const WindowParams &p, int t0) {
   if (c1 != c0 && in) mine = span_at(p.s, count_le_lane(p.s, r.i, c0, c1), r.i);
   in = in && mine.start <= r.i;
   r.start = in ? mine.start : r.i + 1;
-  r.wmin = t0 + (threadIdx.x >> 6) * 32;
+  r.wmin = t0 + wave_id() * 32;
   r.wmax = r.wmin + 31;
   const int lo = r.i - p.window + 1 > r.start ? r.i - p.window + 1 : r.start;
   r.wlo = wave_min(lo);
@@ -93,49 +97,79 @@ struct KeyTiles {
   }
 };
 
-// Adds what the products left out: streamed values that are not finite and visible.  nan: as NaN (the
-// factor may be zero or have either sign), else as they are (the factor is a positive weight).
-template <typename T, int D, int NT, typename F>
-__device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, int row0, bool nan, F seen) {
+// A tile with values that are not finite (rare) is cleaned before it is multiplied, since a masked row's weight of
+// zero would not keep them out; what the lane's own row sees of them is added here first.
+// By element: as they are, for products whose weights are positive.
+template <typename T, int D, int NT> __device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
   const int h8 = (lane_id() >> 5) * 8;
 #pragma unroll 1
-  for (int j = 0; j < 32; ++j) {
-    if (!seen(j)) continue;
-    int row = row0 + j;
+  for (int j = 0; j < WA_TILE; ++j) {
+    const bool on = seen(j);
+    int row = j;
     asm volatile("" : "+v"(row));  // keeps the addresses below out of the registers of the main path
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float x = tile_elem<T, D>(tile, row, t * 32 + 16 * (r >> 3) + h8 + (r & 7));
-        if (!finite(x)) acc[t][r] += nan ? x - x : x;
+        acc[t][r] += on && !finite(x) ? x : 0.f;
         if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);
       }
   }
 }
-
-template <typename T, int D>
-__device__ inline void load_own(Frag<T> (&f)[D / 16], const Rows &rows, int head, int row, bool in) {
-  const T *p = head_of<T>(rows, head) + (int64_t)row * rows.row;
+// By row: NaN for every element, where the weight itself depends on such a value.
+template <typename T, int D, int NT> __device__ inline void mark_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
+  bool bad = false;
+#pragma unroll 1
+  for (int j = 0; j < WA_TILE; ++j) {
+    bool any = false;
+    for (int d = lane_id(); d < D; d += 64) any |= !finite(tile_elem<T, D>(tile, j, d));
+    bad |= __any(any) & seen(j);
+  }
+  const float x = bad ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
-  for (int b = 0; b < D / 16; ++b)
-    f[b] = in ? load8(p, 16 * b + 8 * (lane_id() >> 5), rows.dim, rows.vec) : zero_frag<Frag<T>>();
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[t][r] += x;
 }
+
+// acc += (32 rows of the tile)^T w, for the lane's column of weights.
 template <typename T, int D, int NT>
-__device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &rows, int head, int row, bool in) {
-  if (!in) return;
-  T *p = (T *)rows.p + (int64_t)head * rows.head + (int64_t)row * rows.row;
+__device__ inline void add_rows(f32x16 (&acc)[NT], const T *tile, int row0, const f32x16 &w) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const Frag<T> wf = operand<T>(w, b);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const Frag<T> f = col_frag<D>(tile, row0 + 16 * b, t * 32);
+      acc[t] = mma(f, wf, acc[t]);
+    }
+  }
+}
+
+// The lane's own row, row `r` of the buffer.  Rows of no series (in = false) are zeros.
+template <typename T, int D, bool VEC>
+__device__ inline void load_own(Frag<T> (&f)[D / 16], const Rows &rows, Run buf, int r, bool in) {
+  const uint32_t at = in ? (uint32_t)r * (uint32_t)rows.row * (uint32_t)sizeof(T) : kOutside;
+  const int h8 = 8 * (lane_id() >> 5), dim = in ? rows.dim : 0;
+#pragma unroll
+  for (int b = 0; b < D / 16; ++b) f[b] = buffer_load8<T>(buf, at, 16 * b + h8, dim, VEC);
+}
+template <typename T, int D, bool VEC, int NT>
+__device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &rows, Run buf, int r) {
+  const uint32_t at = (uint32_t)r * (uint32_t)rows.row * (uint32_t)sizeof(T);
+  const int h8 = 8 * (lane_id() >> 5);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     f32x16 c = acc[t];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) c[r] *= by;
+    for (int x = 0; x < 16; ++x) c[x] *= by;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) store8(p, t * 32 + 16 * b + 8 * (lane_id() >> 5), rows.dim, rows.vec, operand<T>(c, b));
+    for (int b = 0; b < 2; ++b) buffer_store8(buf, at, t * 32 + 16 * b + h8, rows.dim, VEC, operand<T>(c, b));
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_forward_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.heads);
   if (item < 0) return;
@@ -147,55 +181,65 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   const QueryRows r = query_rows(p, t0);
   const KeyTiles tl(p, r, t0);
-  const Seen seen = {p.window, p.sinks};
   const int h8 = (lane_id() >> 5) * 8;
   const bool in = r.start <= r.i;
+  const int own = p.s.n - t0 < WA_OWN ? p.s.n - t0 : WA_OWN;
   Frag<T> qf[D / 16];
-  load_own<T, D>(qf, p.q, head, r.i, in);
+  load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
   f32x16 acc[D / 32];
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * kLog2e;
-  const T *kp = head_of<T>(p.k, kv), *vp = head_of<T>(p.v, kv);
-  Staged<T, D, WA_TILE, WA_THREADS> ks, vs;
-  ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(0), 1, tl.rows(0));
-  vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(0), 1, tl.rows(0));
+  Staged<T, D, WA_TILE, WA_THREADS, VEC> ks, vs;
+  ks.load(p.k, kv, tl.first(0), false, tl.rows(0));
+  vs.load(p.v, kv, tl.first(0), false, tl.rows(0));
   for (int t = 0; t < tl.count; ++t) {
     const int j0 = tl.first(t), j1 = tl.end(t);
     __syncthreads();
     ks.store(kt);
-    if (vs.store(vt)) flag[t & 1] = 1;
+    vs.store(vt);
+    if (vs.dirty()) flag[t & 1] = 1;
     if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
     __syncthreads();
-    if (t + 1 < tl.count) {
-      ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(t + 1), 1, tl.rows(t + 1));
-      vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+    // (rows behind part 0 are part 1's; x counts from the tile's first row)
+    const int last = min_of(r.i, j1 - 1) - j0;
+    const Seen seen = {max_of(r.i - p.window + 1, r.start) - j0, last, r.start - j0, min_of(r.start + p.sinks - 1 - j0, last)};
+    if (__builtin_expect(flag[t & 1], 0)) {
+      add_not_finite<T, D>(acc, vt, seen);
+      __syncthreads();
+      vs.clean();
+      vs.store(vt);
+      __syncthreads();
     }
-    const bool dirty = flag[t & 1];
+    if (t + 1 < tl.count) {
+      ks.load(p.k, kv, tl.first(t + 1), false, tl.rows(t + 1));
+      vs.load(p.v, kv, tl.first(t + 1), false, tl.rows(t + 1));
+    }
     if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;  // none of the wave's
     const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
-    // (rows behind part 0 are part 1's)
-    auto visible = [&](int j) { return j < j1 && seen(r.i, j, r.start); };
     f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int b = 0; b < D / 16; ++b)
 #pragma unroll
-      for (int b = 0; b < D / 16; ++b)
+      for (int u = 0; u < 2; ++u)
         s[u] = mma(row_frag<D>(kt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
-    if (!full)
+    if (!full) {
+      asm volatile("");  // (a branch, not selects: most tiles need none)
+      const Seen mine = seen.from(h8);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if (!visible(j0 + u * 32 + 16 * (x >> 3) + h8 + (x & 7))) s[u][x] = -INFINITY;
+        for (int x = 0; x < 16; ++x) s[u][x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[u][x] : -INFINITY;
+    }
     float top = s[0][0];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
     top = fmaxf(top, other_half(top)) * c;
-    if (__any(top > m)) {
+    // (kept while no weight exceeds 2^8: the factor cancels in the end)
+    if (__any(top > m + 8.f)) {
       const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
       m = nm;
       l *= by;
@@ -212,32 +256,19 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
         s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
         l += s[u][x];
       }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const Frag<T> pf = operand<T>(s[u], b);
-#pragma unroll
-        for (int t2 = 0; t2 < D / 32; ++t2) {
-          Frag<T> vf = col_frag<D>(vt, u * 32 + 16 * b, t2 * 32);
-          if (dirty) vf = cleaned(vf);
-          acc[t2] = mma(vf, pf, acc[t2]);
-        }
-      }
-      if (dirty)
-        add_not_finite<T, D>(acc, vt, u * 32, false, [&](int j) { return visible(j0 + u * 32 + j); });
-    }
+    add_rows<T, D>(acc, vt, 0, s[0]);
+    add_rows<T, D>(acc, vt, 32, s[1]);
   }
   l += other_half(l);
   // a row of no series gets zeros
   const float by = in ? 1.f / l : 0.f;
-  store_own<T, D>(acc, by, p.out, head, r.i, r.i < p.s.n);
+  store_own<T, D, VEC>(acc, by, p.out, rows_buffer<T>(p.out, head, t0, own), r.i - t0);
   if (p.lse && r.i < p.s.n && lane_id() < 32)
     p.lse[(int64_t)r.i * p.heads + head] = in ? (m + log2_hw(l)) * kLn2 : -INFINITY;
 }
 
 // dq, and do.o for the kernel that follows.
-template <typename T, int D>
+template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_dq_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.heads);
   if (item < 0) return;
@@ -249,12 +280,12 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   const QueryRows r = query_rows(p, t0);
   const KeyTiles tl(p, r, t0);
-  const Seen seen = {p.window, p.sinks};
   const int h8 = (lane_id() >> 5) * 8;
   const bool in = r.start <= r.i;
+  const int own = p.s.n - t0 < WA_OWN ? p.s.n - t0 : WA_OWN;
   Frag<T> qf[D / 16], of[D / 16];
-  load_own<T, D>(of, p.out, head, r.i, in);
-  load_own<T, D>(qf, p.dout, head, r.i, in);
+  load_own<T, D, VEC>(of, p.out, rows_buffer<T>(p.out, head, t0, own), r.i - t0, in);
+  load_own<T, D, VEC>(qf, p.dout, rows_buffer<T>(p.dout, head, t0, own), r.i - t0, in);
   float delta = 0.f;
 #pragma unroll
   for (int b = 0; b < D / 16; ++b)
@@ -264,32 +295,39 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   if (r.i < p.s.n && lane_id() < 32) p.delta[(int64_t)r.i * p.heads + head] = delta;
 #pragma unroll
   for (int b = 0; b < D / 16; ++b) of[b] = qf[b];
-  load_own<T, D>(qf, p.q, head, r.i, in);
+  load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
   const float lse2 = in ? p.lse[(int64_t)r.i * p.heads + head] * kLog2e : 0.f;
   f32x16 acc[D / 32];
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
   const float c = p.scale * kLog2e;
-  const T *kp = head_of<T>(p.k, kv), *vp = head_of<T>(p.v, kv);
-  Staged<T, D, WA_TILE, WA_THREADS> ks, vs;
-  ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(0), 1, tl.rows(0));
-  vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(0), 1, tl.rows(0));
+  Staged<T, D, WA_TILE, WA_THREADS, VEC> ks, vs;
+  ks.load(p.k, kv, tl.first(0), false, tl.rows(0));
+  vs.load(p.v, kv, tl.first(0), false, tl.rows(0));
   for (int t = 0; t < tl.count; ++t) {
     const int j0 = tl.first(t), j1 = tl.end(t);
     __syncthreads();
-    if (ks.store(kt)) flag[t & 1] = 1;
+    ks.store(kt);
     vs.store(vt);
+    if (ks.dirty()) flag[t & 1] = 1;
     if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
     __syncthreads();
-    if (t + 1 < tl.count) {
-      ks.load(kp, p.k.row, p.k.dim, p.k.vec, tl.first(t + 1), 1, tl.rows(t + 1));
-      vs.load(vp, p.v.row, p.v.dim, p.v.vec, tl.first(t + 1), 1, tl.rows(t + 1));
+    // (rows behind part 0 are part 1's; x counts from the tile's first row)
+    const int last = min_of(r.i, j1 - 1) - j0;
+    const Seen seen = {max_of(r.i - p.window + 1, r.start) - j0, last, r.start - j0, min_of(r.start + p.sinks - 1 - j0, last)};
+    if (__builtin_expect(flag[t & 1], 0)) {
+      mark_not_finite<T, D>(acc, kt, seen);
+      __syncthreads();
+      ks.clean();
+      ks.store(kt);
+      __syncthreads();
     }
-    const bool dirty = flag[t & 1];
+    if (t + 1 < tl.count) {
+      ks.load(p.k, kv, tl.first(t + 1), false, tl.rows(t + 1));
+      vs.load(p.v, kv, tl.first(t + 1), false, tl.rows(t + 1));
+    }
     if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;
     const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
-    // (rows behind part 0 are part 1's)
-    auto visible = [&](int j) { return j < j1 && seen(r.i, j, r.start); };
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s = zero16(), dp = zero16();
@@ -301,23 +339,18 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const float w = exp2_hw(__builtin_fmaf(s[x], c, -lse2)) * (dp[x] - delta);
-        s[x] = full || visible(j0 + u * 32 + 16 * (x >> 3) + h8 + (x & 7)) ? w : 0.f;
+        s[x] = w;
       }
+      if (!full) {
+        asm volatile("");
+        const Seen mine = seen.from(h8);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const Frag<T> pf = operand<T>(s, b);
-#pragma unroll
-        for (int t2 = 0; t2 < D / 32; ++t2) {
-          Frag<T> kf = col_frag<D>(kt, u * 32 + 16 * b, t2 * 32);
-          if (dirty) kf = cleaned(kf);
-          acc[t2] = mma(kf, pf, acc[t2]);
-        }
+        for (int x = 0; x < 16; ++x) s[x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[x] : 0.f;
       }
-      if (dirty)
-        add_not_finite<T, D>(acc, kt, u * 32, true, [&](int j) { return visible(j0 + u * 32 + j); });
+      add_rows<T, D>(acc, kt, u * 32, s);
     }
   }
-  store_own<T, D>(acc, p.scale, p.dq, head, r.i, r.i < p.s.n);
+  store_own<T, D, VEC>(acc, p.scale, p.dq, rows_buffer<T>(p.dq, head, t0, own), r.i - t0);
 }
 
 // Last query row + 1 whose pairs with the key rows of tile [j0, j0 + WA_OWN) the main dk/dv kernel adds:
@@ -333,13 +366,13 @@ __device__ inline int last_query(const WindowParams &p, int j0, bool sinks) {
 // dk and dv: a block owns key rows and streams the query rows that see them, head after head of the
 // group that shares them.  SINK: the rows that stay visible, against the query rows of one section
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
-template <typename T, int D, bool SINK>
+template <typename T, int D, bool VEC, bool SINK>
 __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.kv_heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
   const int kv = item / tiles, tile = item % tiles;
-  const int wave = threadIdx.x >> 6, lane = lane_id(), h8 = (lane >> 5) * 8;
+  const int wave = wave_id(), lane = lane_id(), h8 = (lane >> 5) * 8;
   __shared__ __align__(16) T qt[WA_TILE * D], dt[WA_TILE * D];
   __shared__ float lse_t[WA_TILE], delta_t[WA_TILE];
   __shared__ int flag[2];
@@ -378,23 +411,24 @@ __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kerne
     if (i1 > reach) i1 = reach > j1 ? reach : j1;
     if (i1 < j1) i1 = j1;
   }
-  const Seen seen = {p.window, p.sinks};
   const bool in = end > j;
   Frag<T> kf[D / 16], vf[D / 16];
-  load_own<T, D>(kf, p.k, kv, j, in);
-  load_own<T, D>(vf, p.v, kv, j, in);
+  // the block's own rows, from j_first on (a series' first rows may be fewer than 32)
+  const int j_first = SINK ? start : tile * WA_OWN, own = p.s.n - j_first < WA_OWN ? p.s.n - j_first : WA_OWN;
+  load_own<T, D, VEC>(kf, p.k, rows_buffer<T>(p.k, kv, j_first, own), j - j_first, in);
+  load_own<T, D, VEC>(vf, p.v, rows_buffer<T>(p.v, kv, j_first, own), j - j_first, in);
   f32x16 dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) { dk[t] = zero16(); dv[t] = zero16(); }
   const float c = p.scale * kLog2e;
   const int per_head = (i1 - i0 + WA_TILE - 1) / WA_TILE, count = per_head * group;
-  Staged<T, D, WA_TILE, WA_THREADS> qs, ds;
+  Staged<T, D, WA_TILE, WA_THREADS, VEC> qs, ds;
   float lse_n = 0.f, delta_n = 0.f;
   auto fetch = [&](int t) {
     const int head = kv * group + t / per_head, first = i0 + t % per_head * WA_TILE;
     const int rows = i1 - first < WA_TILE ? i1 - first : WA_TILE;
-    qs.load(head_of<T>(p.q, head), p.q.row, p.q.dim, p.q.vec, first, 1, rows);
-    ds.load(head_of<T>(p.dout, head), p.dout.row, p.dout.dim, p.dout.vec, first, 1, rows);
+    qs.load(p.q, head, first, false, rows);
+    ds.load(p.dout, head, first, false, rows);
     if (threadIdx.x < WA_TILE && (int)threadIdx.x < rows) {
       const int64_t at = (int64_t)(first + threadIdx.x) * p.heads + head;
       lse_n = p.lse[at] * kLog2e;
@@ -402,24 +436,41 @@ __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kerne
     }
   };
   if (count > 0) fetch(0);
-  const int wmin_j = j - (lane & 31), wmax_j = wmin_j + 31;
-  const int wend = wave_max(end), wfrom = wave_min(from);
+  const int wmin_j = SINK ? start : tile * WA_OWN + wave * 32, wmax_j = wmin_j + 31;
+  // of the wave: last series end, first query row of any, and what all have in common
+  const int wend = wave_max(end), wfrom = SINK ? wave_max(from) : 0, wfirst = SINK ? wave_min(from) : 0;
+  const int wlast = min_of(wave_min(end), i1);
+  const bool wall = __all(in);
   for (int t = 0; t < count; ++t) {
     const int r0 = i0 + t % per_head * WA_TILE;
     __syncthreads();
-    bool bad = qs.store(qt);
-    bad |= ds.store(dt) != 0;
-    if (bad) flag[t & 1] = 1;
+    qs.store(qt);
+    ds.store(dt);
+    if (qs.dirty() || ds.dirty()) flag[t & 1] = 1;
     if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
     if (threadIdx.x < WA_TILE) { lse_t[threadIdx.x] = lse_n; delta_t[threadIdx.x] = delta_n; }
     __syncthreads();
+    // query rows [first, last] of a tile see key row j: those of its window, all behind it if it stays visible
+    const int last = min_of(end, i1) - 1 - r0;
+    const Seen seen = {max_of(j, from) - r0, min_of(j < start + p.sinks ? last : j + p.window - 1 - r0, last), 0, -1};
+    if (__builtin_expect(flag[t & 1], 0)) {
+      if (!SINK || wave == 0) {  // (two waves share a section's rows: the first speaks for both)
+        add_not_finite<T, D>(dv, dt, seen);
+        mark_not_finite<T, D>(dk, qt, seen);
+      }
+      __syncthreads();
+      qs.clean();
+      qs.store(qt);
+      ds.clean();
+      ds.store(dt);
+      __syncthreads();
+    }
     if (t + 1 < count) fetch(t + 1);
-    const bool dirty = flag[t & 1];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int ru = r0 + u * 32;
       if (SINK) {
-        if (wave != u || ru + 32 <= wfrom) continue;  // two waves share the section's rows
+        if (wave != u || ru + 32 <= wfirst) continue;  // two waves share the section's rows
       } else {
         if (ru + 31 < wmin_j || ru >= wend) continue;
         if (p.sinks == 0 && ru > wmax_j + p.window - 1) continue;
@@ -430,31 +481,25 @@ __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kerne
         s = mma(row_frag<D>(qt, u * 32 + pi_of(lane & 31), 16 * b + h8), kf[b], s);
         dp = mma(row_frag<D>(dt, u * 32 + pi_of(lane & 31), 16 * b + h8), vf[b], dp);
       }
-      auto visible = [&](int i) { return i >= from && i < end && i < i1 && seen(i, j, start); };
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int row = u * 32 + 16 * (x >> 3) + h8 + (x & 7);
-        const bool on = visible(r0 + row);
-        const float w = exp2_hw(__builtin_fmaf(s[x], c, -lse_t[row]));
-        const float g = w * (dp[x] - delta_t[row]);
-        s[x] = on ? w : 0.f;
-        dp[x] = on ? g : 0.f;
+        s[x] = exp2_hw(__builtin_fmaf(s[x], c, -lse_t[row]));
+        dp[x] = s[x] * (dp[x] - delta_t[row]);
       }
+      if (!(wall && ru >= wmax_j && ru >= wfrom && ru + 31 < wlast && ru + 31 < wmin_j + p.window)) {
+        asm volatile("");
+        const Seen mine = seen.from(h8);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const Frag<T> pf = operand<T>(s, b), gf = operand<T>(dp, b);
-#pragma unroll
-        for (int t2 = 0; t2 < D / 32; ++t2) {
-          Frag<T> of = col_frag<D>(dt, u * 32 + 16 * b, t2 * 32), qf = col_frag<D>(qt, u * 32 + 16 * b, t2 * 32);
-          if (dirty) { of = cleaned(of); qf = cleaned(qf); }
-          dv[t2] = mma(of, pf, dv[t2]);
-          dk[t2] = mma(qf, gf, dk[t2]);
+        for (int x = 0; x < 16; ++x) {
+          const int row = u * 32 + 16 * (x >> 3) + (x & 7);
+          const bool on = (row >= mine.lo) & (row <= mine.hi);
+          s[x] = on ? s[x] : 0.f;
+          dp[x] = on ? dp[x] : 0.f;
         }
       }
-      if (dirty) {
-        add_not_finite<T, D>(dv, dt, u * 32, false, [&](int x) { return visible(ru + x); });
-        add_not_finite<T, D>(dk, qt, u * 32, true, [&](int x) { return visible(ru + x); });
-      }
+      add_rows<T, D>(dv, dt, u * 32, s);
+      add_rows<T, D>(dk, qt, u * 32, dp);
     }
   }
   if (SINK) {
@@ -484,8 +529,8 @@ __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kerne
         if (d < p.v.dim) dv[t][x] += o[p.k.dim + d];
       }
   }
-  store_own<T, D>(dk, p.scale, p.dk, kv, j, j < p.s.n);
-  store_own<T, D>(dv, 1.f, p.dv, kv, j, j < p.s.n);
+  store_own<T, D, VEC>(dk, p.scale, p.dk, rows_buffer<T>(p.dk, kv, j_first, own), j - j_first);
+  store_own<T, D, VEC>(dv, 1.f, p.dv, rows_buffer<T>(p.dv, kv, j_first, own), j - j_first);
 }
 
 // Adds up the parts of all sections that a series reaches into, in the place of the first of them.  A
@@ -535,44 +580,50 @@ static int window_check(const tmp_window_attention_args *a, const char *what, bo
   return TMP_OK;
 }
 
-static WindowParams window_params(const tmp_window_attention_args *a) {
-  WindowParams p;
-  memset(&p, 0, sizeof(p));
+static int window_params(const tmp_window_attention_args *a, const char *what, bool grad, WindowParams *p) {
+  memset(p, 0, sizeof(*p));
   const int b = a->type == TMP_F32 ? 4 : 2;
-  p.s.offsets = a->offsets; p.s.n_series = a->n_series; p.s.n = (int32_t)a->n;
-  p.q = rows_of(a->q, a->dim_k, b); p.k = rows_of(a->k, a->dim_k, b); p.v = rows_of(a->v, a->dim_v, b);
-  p.out = rows_of(a->out, a->dim_v, b); p.dout = rows_of(a->dout, a->dim_v, b);
-  p.dq = rows_of(a->dq, a->dim_k, b); p.dk = rows_of(a->dk, a->dim_k, b); p.dv = rows_of(a->dv, a->dim_v, b);
-  p.lse = a->lse;
-  p.heads = a->heads; p.kv_heads = a->kv_heads; p.sinks = a->sinks; p.scale = a->scale;
-  p.window = (int32_t)(a->window < a->n ? a->window : a->n);
-  return p;
+  p->s.offsets = a->offsets; p->s.n_series = a->offsets ? a->n_series : 1; p->s.n = (int32_t)a->n;
+  TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p->q);
+  TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p->k);
+  TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p->v);
+  TMP_ROWS(what, a->out, a->n, a->dim_v, b, &p->out);
+  if (grad) {
+    TMP_ROWS(what, a->dout, a->n, a->dim_v, b, &p->dout);
+    TMP_ROWS(what, a->dq, a->n, a->dim_k, b, &p->dq);
+    TMP_ROWS(what, a->dk, a->n, a->dim_k, b, &p->dk);
+    TMP_ROWS(what, a->dv, a->n, a->dim_v, b, &p->dv);
+  }
+  p->lse = a->lse;
+  p->heads = a->heads; p->kv_heads = a->kv_heads; p->sinks = a->sinks; p->scale = a->scale;
+  p->window = (int32_t)(a->window < a->n ? a->window : a->n);
+  return TMP_OK;
 }
 
-template <typename T, int D> static void window_forward(const WindowParams &p, hipStream_t st) {
+template <typename T, int D, bool VEC> static void window_forward(const WindowParams &p, hipStream_t st) {
   const int tiles = (p.s.n + WA_OWN - 1) / WA_OWN;
   ProfScope ps("window_forward_kernel", st);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_forward_kernel<T, D>), dim3(grid_of_items((int64_t)tiles * p.heads)),
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_forward_kernel<T, D, VEC>), dim3(grid_of_items((int64_t)tiles * p.heads)),
                      dim3(WA_THREADS), 0, st, p, tiles);
 }
 
-template <typename T, int D> static void window_grad(const WindowParams &p, hipStream_t st) {
+template <typename T, int D, bool VEC> static void window_grad(const WindowParams &p, hipStream_t st) {
   const int tiles = (p.s.n + WA_OWN - 1) / WA_OWN, sections = (p.s.n + WA_SECTION - 1) / WA_SECTION;
   {
     ProfScope ps("window_dq_kernel", st);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dq_kernel<T, D>), dim3(grid_of_items((int64_t)tiles * p.heads)),
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dq_kernel<T, D, VEC>), dim3(grid_of_items((int64_t)tiles * p.heads)),
                        dim3(WA_THREADS), 0, st, p, tiles);
   }
   if (p.sinks > 0 && sections > 1) {
     {
       ProfScope ps("window_dkdv_kernel(sinks)", st);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, true>), dim3(grid_of_items((int64_t)sections * p.kv_heads)),
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, VEC, true>), dim3(grid_of_items((int64_t)sections * p.kv_heads)),
                          dim3(WA_THREADS), 0, st, p, sections);
     }
     TMP_LAUNCH(sink_sum_kernel, dim3(sections * p.kv_heads), dim3(256), st, p);
   }
   ProfScope ps("window_dkdv_kernel", st);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, false>), dim3(grid_of_items((int64_t)tiles * p.kv_heads)),
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(window_dkdv_kernel<T, D, VEC, false>), dim3(grid_of_items((int64_t)tiles * p.kv_heads)),
                      dim3(WA_THREADS), 0, st, p, tiles);
 }
 
@@ -587,19 +638,6 @@ static void window_plan(const tmp_window_attention_args *a, Workspace &ws, Windo
                                     ? (size_t)sections * 2 * a->kv_heads * a->sinks * (a->dim_k + a->dim_v) : 1);
 }
 
-#define TMP_BY_TYPE_AND_DIM(fn, type, d, ...)                                        \
-  do {                                                                               \
-    if ((type) == TMP_F32) {                                                         \
-      if ((d) == 32) fn<float, 32>(__VA_ARGS__);                                     \
-      else if ((d) == 64) fn<float, 64>(__VA_ARGS__);                                \
-      else fn<float, 128>(__VA_ARGS__);                                              \
-    } else {                                                                         \
-      if ((d) == 32) fn<__bf16, 32>(__VA_ARGS__);                                    \
-      else if ((d) == 64) fn<__bf16, 64>(__VA_ARGS__);                               \
-      else fn<__bf16, 128>(__VA_ARGS__);                                             \
-    }                                                                                \
-  } while (0)
-
 }  // namespace tmp
 
 using namespace tmp;
@@ -608,9 +646,11 @@ extern "C" int tmp_window_attention(const tmp_window_attention_args *a, void *st
   clear_error();
   TMP_TRY(window_check(a, "tmp_window_attention", false));
   if (a->n == 0) return TMP_OK;
-  const WindowParams p = window_params(a);
+  WindowParams p;
+  TMP_TRY(window_params(a, "tmp_window_attention", false, &p));
   const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
-  TMP_BY_TYPE_AND_DIM(window_forward, a->type, d, p, (hipStream_t)stream);
+  const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec;
+  TMP_BY_FORM(window_forward, a->type, d, vec, p, (hipStream_t)stream);
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
 }
@@ -628,7 +668,8 @@ extern "C" int tmp_window_attention_grad(const tmp_window_attention_args *a, voi
   clear_error();
   TMP_TRY(window_check(a, "tmp_window_attention_grad", true));
   if (a->n == 0) return TMP_OK;
-  WindowParams p = window_params(a);
+  WindowParams p;
+  TMP_TRY(window_params(a, "tmp_window_attention_grad", true, &p));
   Workspace ws(workspace, workspace_bytes);
   WindowPlan w;
   window_plan(a, ws, &w);
@@ -636,7 +677,8 @@ extern "C" int tmp_window_attention_grad(const tmp_window_attention_args *a, voi
   p.delta = w.delta;
   p.sink_part = w.sink_part;
   const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
-  TMP_BY_TYPE_AND_DIM(window_grad, a->type, d, p, (hipStream_t)stream);
+  const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec && p.dout.vec && p.dq.vec && p.dk.vec && p.dv.vec;
+  TMP_BY_FORM(window_grad, a->type, d, vec, p, (hipStream_t)stream);
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
 }
