@@ -17,6 +17,7 @@ are differentiable in q, k and v (decay_attention in `state` too); `*_grad` are 
 themselves, for programs that do not use autograd or capture a training step into a graph.  `*_step` add one row
 to each of some slots of kept state.  Calls do not wait for the device.
 """
+import contextlib
 import ctypes as C
 
 import torch
@@ -37,6 +38,11 @@ def _on_device(t, name, device=None):
 
 def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
     """[rows, heads, dim], innermost dimension contiguous; type and device of `like`."""
+    if like is not None and isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.device == like.device and t.dim() == 3:
+        have, last = t.shape, t.stride()[2]  # the usual case, asked for at once: small calls are bound by their host part
+        if have[0] == n and (heads is None or have[1] == heads) and (dim is None or have[2] == dim) and last == 1:
+            if have[1] and have[2]:
+                return t
     _on_device(t, name, None if like is None else like.device)
     if t.dtype not in _TYPES:
         raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
@@ -79,7 +85,8 @@ def _scale(scale, dim):
 
 
 def _ref(t):
-    return RowsRef(None, 0, 0) if t is None else RowsRef(t.data_ptr(), t.stride(0), t.stride(1))
+    row, head, _ = t.stride()
+    return RowsRef(t.data_ptr(), row, head)
 
 
 def _p(t):
@@ -87,7 +94,12 @@ def _p(t):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _current(device):
+    """The device's context, entered only where it is not the current one already."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _workspace(nbytes, device):
@@ -131,7 +143,7 @@ def _decay_args(q, k, v, log_decay, offsets, scale, state):
 
 
 def _decay_call(fn, a, device):
-    with torch.cuda.device(device):
+    with _current(device):
         ws = _workspace(lib().tmp_decay_attention_workspace_bytes(C.byref(a)), device)
         check(getattr(lib(), fn)(C.byref(a), ws.data_ptr(), ws.numel(), _stream(device)), fn)
 
@@ -208,9 +220,9 @@ def _slots_check(slots, n, n_slots, device):
 
 
 def _no_grad(**tensors):
-    if torch.is_grad_enabled():
-        for name, t in tensors.items():
-            if t.requires_grad:
+    for name, t in tensors.items():
+        if t.requires_grad:
+            if torch.is_grad_enabled():
                 raise ValueError(f"{name} requires a gradient; a step has none (use the form over whole series)")
 
 
@@ -234,7 +246,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     a = DecayAttentionStepArgs(n=n, n_slots=state.shape[0], slots=_p(slots), type=_TYPES[q.dtype], heads=heads, dim_k=dk,
                                dim_v=dv, scale=_scale(scale, dk), log_decay=log_decay.data_ptr(), q=_ref(q), k=_ref(k),
                                v=_ref(v), out=_ref(out), state=state.data_ptr())
-    with torch.cuda.device(q.device):
+    with _current(q.device):
         check(lib().tmp_decay_attention_step(C.byref(a), _stream(q.device)), "tmp_decay_attention_step")
     return out
 
@@ -260,7 +272,7 @@ def _window_forward(q, k, v, window, sinks, offsets, scale, return_lse):
     out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device) if return_lse else None
     a.out, a.lse = _ref(out), _p(lse)
-    with torch.cuda.device(q.device):
+    with _current(q.device):
         check(lib().tmp_window_attention(C.byref(a), _stream(q.device)), "tmp_window_attention")
     return out, lse
 
@@ -274,7 +286,7 @@ def window_attention_grad(dout, q, k, v, out, lse, window, sinks=0, offsets=None
     _plain_check(lse, "lse", torch.float32, (n, heads), q.device)
     gq, gk, gv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     a.out, a.lse, a.dout, a.dq, a.dk, a.dv = _ref(out), lse.data_ptr(), _ref(dout), _ref(gq), _ref(gk), _ref(gv)
-    with torch.cuda.device(q.device):
+    with _current(q.device):
         ws = _workspace(lib().tmp_window_attention_grad_workspace_bytes(C.byref(a)), q.device)
         check(lib().tmp_window_attention_grad(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q.device)),
               "tmp_window_attention_grad")
@@ -353,7 +365,7 @@ def window_cache_write(k, v, k_cache, v_cache, length, sinks=0, offsets=None, sl
     a = WindowCacheWriteArgs(n=n, n_series=n_series, offsets=_p(offsets), n_slots=n_slots, slots=_p(slots),
                              type=_TYPES[k.dtype], kv_heads=kv, dim_k=dk, dim_v=dv, window=window, sinks=sinks, k=_ref(k),
                              v=_ref(v), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache), length=length.data_ptr())
-    with torch.cuda.device(k.device):
+    with _current(k.device):
         check(lib().tmp_window_cache_write(C.byref(a), _stream(k.device)), "tmp_window_cache_write")
 
 
@@ -378,7 +390,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
                                 dim_k=dk, dim_v=dv, window=window, sinks=sinks, scale=_scale(scale, dk), q=_ref(q), k=_ref(k),
                                 v=_ref(v), out=_ref(out), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache),
                                 length=length.data_ptr())
-    with torch.cuda.device(q.device):
+    with _current(q.device):
         ws = _workspace(lib().tmp_window_attention_step_workspace_bytes(C.byref(a)), q.device)
         check(lib().tmp_window_attention_step(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q.device)),
               "tmp_window_attention_step")

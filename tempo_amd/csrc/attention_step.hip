@@ -228,9 +228,11 @@ __global__ __launch_bounds__(256, D * sizeof(T) >= 512 ? 1 : 2) void window_step
 }
 
 // Joins the parts of a (row, head); the first head's block counts the row.
+constexpr int WS_MOST_SPLITS = 2048;
 template <typename T>
 __global__ __launch_bounds__(128) void window_join_kernel(WindowStepParams p) {
-  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, d = threadIdx.x;
+  __shared__ float by[WS_MOST_SPLITS];
+  const int b = blockIdx.x / p.heads, head = blockIdx.x % p.heads, d = threadIdx.x, lane = lane_id();
   const int slot = slot_of(p.slots, b, p.n_slots);
   T *o = (T *)p.out.p + (int64_t)head * p.out.head + (int64_t)b * p.out.row;
   const int width = p.v.dim + 2;
@@ -240,15 +242,32 @@ __global__ __launch_bounds__(128) void window_join_kernel(WindowStepParams p) {
     return;
   }
   float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, in[s * width + p.v.dim]);
-  float sum = 0.f, weights = 0.f;
+  for (int s = lane; s < p.splits; s += 64) top = fmaxf(top, in[s * width + p.v.dim]);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   const float mm = top > -INFINITY ? top : 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float by = exp2_hw(in[s * width + p.v.dim] - mm);
-    weights = __builtin_fmaf(by, in[s * width + p.v.dim + 1], weights);
-    if (d < p.v.dim) sum = __builtin_fmaf(by, in[s * width + d], sum);
+  float weights = 0.f;
+  for (int s = lane; s < p.splits; s += 64) {
+    const float e = exp2_hw(in[s * width + p.v.dim] - mm);
+    weights = __builtin_fmaf(e, in[s * width + p.v.dim + 1], weights);
+    by[s] = e;  // (both waves write the same)
   }
-  if (d < p.v.dim) o[d] = (T)(sum / weights);
+#pragma unroll
+  for (int x = 32; x; x >>= 1) weights += __shfl_xor(weights, x);
+  __syncthreads();
+  if (d < p.v.dim) {
+    float sum = 0.f;
+    int s = 0;
+    for (; s + 8 <= p.splits; s += 8) {
+      float x[8];
+#pragma unroll
+      for (int a = 0; a < 8; ++a) x[a] = in[(s + a) * width + d];
+#pragma unroll
+      for (int a = 0; a < 8; ++a) sum = __builtin_fmaf(by[s + a], x[a], sum);
+    }
+    for (; s < p.splits; ++s) sum = __builtin_fmaf(by[s], in[s * width + d], sum);
+    o[d] = (T)(sum / weights);
+  }
   if (head == 0 && d == 0) {
     const int64_t t = p.length[slot];
     p.length[slot] = t < 0 ? 1 : t + 1;
@@ -349,7 +368,7 @@ static int window_step_check(const tmp_window_attention_step_args *a, const char
 static void window_step_split(const tmp_window_attention_step_args *a, int *splits, int *chunk) {
   const int64_t cap = (int64_t)a->window + a->sinks, group = a->heads / a->kv_heads;
   const int64_t units = (a->n > 0 ? a->n : 1) * a->kv_heads * ((group + 31) / 32);
-  int64_t want = (2048 + units - 1) / units;
+  int64_t want = (WS_MOST_SPLITS + units - 1) / units;
   int64_t rows = (cap + want - 1) / want;
   rows = (rows + 31) / 32 * 32;
   *chunk = (int)rows;

@@ -367,7 +367,7 @@ __device__ inline int last_query(const WindowParams &p, int j0, bool sinks) {
 // group that shares them.  SINK: the rows that stay visible, against the query rows of one section
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
 template <typename T, int D, bool VEC, bool SINK>
-__global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
+__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.kv_heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
@@ -503,30 +503,34 @@ __global__ __launch_bounds__(WA_THREADS, D >= 64 ? 1 : 2) void window_dkdv_kerne
     }
   }
   if (SINK) {
-    if (wave > 1 || (lane & 31) >= p.sinks) return;
-    const int width = p.k.dim + p.v.dim;
-    float *o = p.sink_part + ((((int64_t)tile * 2 + wave) * p.kv_heads + kv) * p.sinks + (lane & 31)) * width;
+    if (wave > 1) return;
+    const int width = p.k.dim + p.v.dim, at = (lane & 31) * width;  // (rows behind the sinks are behind the buffer's end)
+    const Buffer o = buffer_of(p.sink_part + (((int64_t)tile * 2 + wave) * p.kv_heads + kv) * p.sinks * width, p.sinks * width * 4);
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int d = t * 32 + 16 * (x >> 3) + h8 + (x & 7);
-        if (d < p.k.dim) o[d] = dk[t][x];
-        if (d < p.v.dim) o[p.k.dim + d] = dv[t][x];
+        const float a = dk[t][x], b = dv[t][x];
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, a), o, d < p.k.dim ? (at + d) * 4 : kOutside, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, b), o, d < p.v.dim ? (at + p.k.dim + d) * 4 : kOutside, 0, 0);
       }
     return;
   }
-  if (p.sinks > 0 && in && j < start + p.sinks && (end - 1) / WA_SECTION > start / WA_SECTION) {
+  const bool more = in && j < start + p.sinks && (end - 1) / WA_SECTION > start / WA_SECTION;
+  if (p.sinks > 0 && __any(more)) {
     // what the sections behind the series' first add, summed up in the place of the first of them
     const int width = p.k.dim + p.v.dim;
-    const float *o = p.sink_part + (((int64_t)(start / WA_SECTION + 1) * 2 * p.kv_heads + kv) * p.sinks + (j - start)) * width;
+    const float *o = p.sink_part + (more ? (((int64_t)(start / WA_SECTION + 1) * 2 * p.kv_heads + kv) * p.sinks + (j - start)) * width : 0);
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const int d = t * 32 + 16 * (x >> 3) + h8 + (x & 7);
-        if (d < p.k.dim) dk[t][x] += o[d];
-        if (d < p.v.dim) dv[t][x] += o[p.k.dim + d];
+        const bool on_k = more & (d < p.k.dim), on_v = more & (d < p.v.dim);
+        const float a = o[on_k ? d : 0], b = o[on_v ? p.k.dim + d : 0];
+        dk[t][x] += on_k ? a : 0.f;
+        dv[t][x] += on_v ? b : 0.f;
       }
   }
   store_own<T, D, VEC>(dk, p.scale, p.dk, rows_buffer<T>(p.dk, kv, j_first, own), j - j_first);
