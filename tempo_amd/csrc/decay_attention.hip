@@ -43,19 +43,9 @@ __device__ inline float power(float log2_decay, int m) { return m == 0 ? 1.f : e
 
 // The series that the row at walk position `pos` lies in, in walk positions.  index -1: a stretch of rows
 // that belong to none.
-__device__ inline Span walk_span(const DecayParams &p, int pos) {
-  const int n = p.s.n, row = p.reverse ? n - 1 - pos : pos;
-  const int c = count_le(p.s, row, 0, p.s.n_series + 1);
-  Span sp = span_at(p.s, c, row);
-  if (sp.start > row) {
-    sp.index = -1;
-    int64_t end = n;
-    if (!p.reverse && c < 1) end = p.s.offsets[0];
-    if (p.reverse && c > p.s.n_series) end = n - p.s.offsets[p.s.n_series];
-    sp.start = pos;
-    sp.end = end > n ? n : end <= pos ? pos + 1 : (int)end;
-    return sp;
-  }
+__device__ inline Span walk_span(const DecayParams &p, Offsets &w, int pos) {
+  const int n = p.s.n;
+  Span sp = span_of(p.s, w, p.reverse ? n - 1 - pos : pos, p.reverse);
   if (p.reverse) {
     const int a = n - sp.end;
     sp.end = n - sp.start;
@@ -141,14 +131,17 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
   const int sec0 = sec * p.section, sec1 = sec0 + p.section < p.s.n ? sec0 + p.section : p.s.n;
   int pos = sec0;
   Span sp;
+  Offsets near = {0, -1};  // (nothing is found in it: filled where it is needed)
+  if (OUT) near = offsets_at(p.s, p.reverse ? p.s.n - 1 - sec0 : sec0, p.reverse);
   if (!OUT) {
-    sp = walk_span(p, sec1 - 1);
+    Offsets last = offsets_at(p.s, p.reverse ? p.s.n - sec1 : sec1 - 1, false);
+    sp = walk_span(p, last, sec1 - 1);
     const bool on = sp.index >= 0 && sp.end > sec1;
     if (head == 0 && threadIdx.x == 0) p.link[sec + 1] = !on ? 0 : sp.start < sec0 ? 2 : 1;
     if (!on) return;
     pos = sp.start > sec0 ? sp.start : sec0;
   } else {
-    sp = walk_span(p, sec0);
+    sp = walk_span(p, near, sec0);
   }
   extern __shared__ __align__(16) unsigned char smem[];
   T *kt = (T *)smem, *vt = kt + DA_PIECE * D, *qt = vt + DA_PIECE * D;
@@ -213,7 +206,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
     Span nsp = sp;
     int nlen = 0;
     if (next < sec1) {
-      if (next >= sp.end) nsp = walk_span(p, next);
+      if (next >= sp.end) nsp = walk_span(p, near, next);
       nlen = length(next, nsp);
       fetch(next, nsp.index < 0 ? 0 : nlen);
     }

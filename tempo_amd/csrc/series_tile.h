@@ -331,20 +331,10 @@ struct Span {
 };
 constexpr int kNoSeries = 0x7fff0000;  // beyond every row: tables have fewer than 2^31 - 65536
 
-__device__ inline Span span_at(const Series &s, int count, int row) {  // count = offsets that are <= row
-  Span sp;
-  if (!s.offsets) { sp.start = 0; sp.end = s.n; sp.index = 0; return sp; }
-  if (count < 1 || count > s.n_series) { sp.start = kNoSeries; sp.end = row + 1; sp.index = -1; return sp; }
-  const int64_t a = s.offsets[count - 1], b = s.offsets[count];
-  sp.start = a < 0 ? 0 : a > row ? row : (int)a;
-  sp.end = b > s.n ? s.n : b <= row ? row + 1 : (int)b;
-  sp.index = count - 1;
-  return sp;
-}
-// How many offsets are <= row, found by all lanes of the wave together, 64 places a step; the answer is
-// known to be in [lo, hi].
-__device__ inline int count_le(const Series &s, int64_t row, int lo, int hi) {
+// How many offsets are <= row, found by all lanes of the wave together, 64 places a step.
+__device__ inline int count_le(const Series &s, int64_t row) {
   if (!s.offsets) return 1;
+  int lo = 0, hi = s.n_series + 1;
   while (lo < hi) {
     const int step = (hi - lo + 63) / 64;
     const int64_t at = (int64_t)lo + (int64_t)(lane_id() + 1) * step - 1;
@@ -356,13 +346,75 @@ __device__ inline int count_le(const Series &s, int64_t row, int lo, int hi) {
   }
   return __builtin_amdgcn_readfirstlane(lo);
 }
-// The same for the lane's own row, between the counts of the tile's first and last rows.
-__device__ inline int count_le_lane(const Series &s, int64_t row, int lo, int hi) {
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (s.offsets[mid] <= row) lo = mid + 1; else hi = mid;
+
+// Sixty-four consecutive offsets, one a lane (-1 before the first, past every row behind the last): the series of
+// near rows are found in them without further loads.
+struct Offsets {
+  int base;  // of lane 0
+  int o;
+};
+__device__ inline Offsets offsets_from(const Series &s, int base) {
+  Offsets w;
+  w.base = base;
+  const int i = base + lane_id();
+  if (!s.offsets) {
+    w.o = i < 0 ? -1 : i == 0 ? 0 : i == 1 ? s.n : kNoSeries;
+  } else {
+    const int64_t x = s.offsets[i < 0 ? 0 : i > s.n_series ? s.n_series : i];
+    w.o = i < 0 ? -1 : i > s.n_series ? kNoSeries : x < 0 ? 0 : x > s.n ? s.n : (int)x;
   }
-  return lo;
+  return w;
+}
+// The window of offsets around `row`, most of it behind (back: before) it.
+__device__ inline Offsets offsets_at(const Series &s, int row, bool back) {
+  const int c = count_le(s, row);
+  return offsets_from(s, back ? c - 62 : c - 1);
+}
+// The series of `row` (the same for all lanes).  A stretch of rows that belong to none has index -1.
+__device__ inline Span span_of(const Series &s, Offsets &w, int row, bool back) {
+  uint64_t past = __ballot(w.o > row);
+  if (past == 0 || (past & 1)) {  // not in the window
+    w = offsets_at(s, row, back);
+    past = __ballot(w.o > row);
+  }
+  // (offsets that do not ascend may leave nothing here: the row then stands alone)
+  const int l = past == 0 || (past & 1) ? -1 : __builtin_ctzll(past);
+  Span sp = {row, row + 1, -1};
+  if (l < 0) return sp;
+  const int a = __builtin_amdgcn_readlane(w.o, l - 1), b = __builtin_amdgcn_readlane(w.o, l);
+  sp.start = a < 0 ? 0 : a;
+  sp.end = b > s.n ? s.n : b;
+  const int i = w.base + l - 1;
+  sp.index = i < 0 || i >= s.n_series ? -1 : i;
+  return sp;
+}
+// The series of each lane's own row, one of [first, last]; the window is the one of `first`.
+__device__ inline Span lane_span(const Series &s, const Offsets &w, int first, int last, int row) {
+  const int l0 = __popcll(__ballot(w.o <= first)), l1 = __popcll(__ballot(w.o <= last));
+  int a, b, i;
+  if (l1 < 64) {
+    int c = l0;
+    for (int l = l0; l < l1; ++l) c += __builtin_amdgcn_readlane(w.o, l) <= row;
+    a = __shfl(w.o, c - 1);
+    b = __shfl(w.o, c);
+    i = w.base + c - 1;
+  } else {  // more series start among these rows than the window holds: each lane looks for its own
+    int lo = w.base < 0 ? 0 : w.base, hi = s.n_series + 1;
+    while (lo < hi) {
+      const int mid = lo + ((hi - lo) >> 1);
+      if (s.offsets[mid] <= row) lo = mid + 1; else hi = mid;
+    }
+    i = lo - 1;
+    const int64_t x = s.offsets[i < 0 ? 0 : i], y = s.offsets[i >= s.n_series ? s.n_series : i + 1];
+    a = (int)(x < 0 ? 0 : x > s.n ? s.n : x);
+    b = (int)(y < 0 ? 0 : y > s.n ? s.n : y);
+  }
+  Span sp = {kNoSeries, row + 1, -1};
+  if (i < 0 || i >= s.n_series || a > row || b <= row) return sp;
+  sp.start = a;
+  sp.end = b;
+  sp.index = i;
+  return sp;
 }
 
 __device__ inline float other_half(float x) { return __shfl_xor(x, 32); }

@@ -53,19 +53,14 @@ struct QueryRows {
 __device__ inline QueryRows query_rows(const WindowParams &p, int t0) {
   QueryRows r;
   const int t1 = t0 + WA_OWN < p.s.n ? t0 + WA_OWN : p.s.n;
-  const int most = p.s.n_series + 1;
-  const int c0 = count_le(p.s, t0, 0, most);
-  int c1 = c0;
-  if (p.s.offsets && c0 < most && p.s.offsets[c0] < t1) c1 = count_le(p.s, t1 - 1, c0, most);
+  Offsets w = offsets_at(p.s, t0, false);
+  const Span first = span_of(p.s, w, t0, false);
   r.i = t0 + wave_id() * 32 + (lane_id() & 31);
-  const Span first = span_at(p.s, c0, t0);
-  r.first_start = first.start < t0 ? first.start : t0;
-  const int w = t0 - p.window + 1;
-  r.lo = w > r.first_start ? w : r.first_start;
-  Span mine = first;
-  bool in = r.i < t1;
-  if (c1 != c0 && in) mine = span_at(p.s, count_le_lane(p.s, r.i, c0, c1), r.i);
-  in = in && mine.start <= r.i;
+  r.first_start = first.index < 0 ? t0 : first.start;
+  const int back = t0 - p.window + 1;
+  r.lo = back > r.first_start ? back : r.first_start;
+  const Span mine = lane_span(p.s, w, t0, t1 - 1, r.i);
+  const bool in = r.i < t1 && mine.start <= r.i;
   r.start = in ? mine.start : r.i + 1;
   r.wmin = t0 + wave_id() * 32;
   r.wmax = r.wmin + 31;
@@ -377,12 +372,12 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   __shared__ float lse_t[WA_TILE], delta_t[WA_TILE];
   __shared__ int flag[2];
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
-  const int most = p.s.n_series + 1;
   int j, start, end, i0, i1, from = 0;  // the lane's key row and its series; query rows [i0, i1), those before `from` left out
   if (SINK) {
     const int sec0 = tile * WA_SECTION;
-    const Span sp = span_at(p.s, count_le(p.s, sec0, 0, most), sec0);
-    if (sp.start >= sec0) return;  // (uniform) no series reaches over the section's start
+    Offsets w = offsets_at(p.s, sec0, false);
+    const Span sp = span_of(p.s, w, sec0, false);
+    if (sp.index < 0 || sp.start >= sec0) return;  // (uniform) no series reaches over the section's start
     j = sp.start + (lane & 31);
     start = sp.start;
     end = (lane & 31) < p.sinks && j < sp.end ? sp.end : j;
@@ -393,22 +388,20 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
     if (j / WA_SECTION >= tile) from = i1;  // (a sink row inside the section itself: all its pairs are the other form's)
   } else {
     const int j0 = tile * WA_OWN, j1 = j0 + WA_OWN < p.s.n ? j0 + WA_OWN : p.s.n;
-    const int c0 = count_le(p.s, j0, 0, most);
-    int c1 = c0;
-    if (p.s.offsets && c0 < most && p.s.offsets[c0] < j1) c1 = count_le(p.s, j1 - 1, c0, most);
+    Offsets w = offsets_at(p.s, j0, false);
+    const Span first = span_of(p.s, w, j0, false);
     j = j0 + wave * 32 + (lane & 31);
-    Span mine = span_at(p.s, c0, j0);
-    if (c1 != c0 && j < j1) mine = span_at(p.s, count_le_lane(p.s, j, c0, c1), j);
+    const Span mine = lane_span(p.s, w, j0, j1 - 1, j);
     const bool in = j < j1 && mine.start <= j;
     start = in ? mine.start : j;
     end = in ? mine.end : j;
     i0 = j0;
-    // every wave looks at the same rows: the last series' sinks decide for the block
-    const Span last = span_at(p.s, c1, j1 - 1), fst = span_at(p.s, c0, j0);
-    const bool sinks = p.sinks > 0 && (c1 != c0 || fst.start + p.sinks > j0);
+    // every wave looks at the same rows: whether the tile holds rows that stay visible, and where the last series ends
+    const Span last = span_of(p.s, w, j1 - 1, false);
+    const bool sinks = p.sinks > 0 && (first.end < j1 || (first.index >= 0 && first.start + p.sinks > j0));
     i1 = last_query(p, j0, sinks);
-    const int reach = last.start <= j1 - 1 ? last.end : j1;
-    if (i1 > reach) i1 = reach > j1 ? reach : j1;
+    const int reach = last.index < 0 ? j1 : last.end;
+    if (i1 > reach) i1 = reach;
     if (i1 < j1) i1 = j1;
   }
   const bool in = end > j;
@@ -542,8 +535,9 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
 __global__ __launch_bounds__(256) void sink_sum_kernel(WindowParams p) {
   const int sec = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
   const int sec0 = sec * WA_SECTION;
-  const Span sp = span_at(p.s, count_le(p.s, sec0, 0, p.s.n_series + 1), sec0);
-  if (sp.start >= sec0 || sp.start / WA_SECTION + 1 != sec) return;
+  Offsets w = offsets_at(p.s, sec0, false);
+  const Span sp = span_of(p.s, w, sec0, false);
+  if (sp.index < 0 || sp.start >= sec0 || sp.start / WA_SECTION + 1 != sec) return;
   const int last = (sp.end - 1) / WA_SECTION;
   const int count = p.sinks * (p.k.dim + p.v.dim);
   const int64_t step = (int64_t)p.kv_heads * count;  // from one part to the next
