@@ -19,7 +19,7 @@ namespace tmp {
 constexpr int WA_OWN = 128;    // rows that a block owns, 32 to each wave
 constexpr int WA_TILE = 64;    // rows of a streamed tile
 constexpr int WA_THREADS = 256;
-constexpr int WA_SECTION = 256;  // rows whose share of the sinks' gradients is added up by one block
+constexpr int WA_SECTION = WA_OWN;  // query rows whose share of the sinks' gradients one block adds up
 
 struct WindowParams {
   Series s;
@@ -48,6 +48,10 @@ struct QueryRows {
   int lo, first_start;        // of the block: first row in any window, start of its first row's series
   int wmin, wmax, wlo, wstart;  // of the wave: first and last row, first row in any window, last start
   bool all;                   // every row of the wave lies in a series
+  // Whether the wave may see any of `rows` rows from j0 on.
+  __device__ inline bool any(const WindowParams &p, int j0, int rows) const {
+    return j0 <= wmax && (j0 + rows > wlo || j0 < wstart + p.sinks);
+  }
 };
 
 __device__ inline QueryRows query_rows(const WindowParams &p, int t0) {
@@ -166,6 +170,8 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
 
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_forward_kernel(WindowParams p, int tiles) {
+  // float: matrix instructions are a sixteenth as fast, and parts that a wave does not see are left out one by one
+  constexpr int PARTS = sizeof(T) == 4 ? 1 : 2;
   const int item = item_of_block(tiles * p.heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
@@ -211,48 +217,55 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
       ks.load(p.k, kv, tl.first(t + 1), false, tl.rows(t + 1));
       vs.load(p.v, kv, tl.first(t + 1), false, tl.rows(t + 1));
     }
-    if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;  // none of the wave's
+    if (!r.any(p, j0, WA_TILE)) continue;
     const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
-    f32x16 s[2] = {zero16(), zero16()};
+    // PARTS parts of 32 rows at a time
 #pragma unroll
-    for (int b = 0; b < D / 16; ++b)
+    for (int u0 = 0; u0 < 2; u0 += PARTS) {
+      if (PARTS == 1 && !r.any(p, j0 + u0 * 32, 32)) continue;
+      f32x16 s[PARTS];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        s[u] = mma(row_frag<D>(kt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
-    if (!full) {
-      asm volatile("");  // (a branch, not selects: most tiles need none)
-      const Seen mine = seen.from(h8);
+      for (int u = 0; u < PARTS; ++u) s[u] = zero16();
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int b = 0; b < D / 16; ++b)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) s[u][x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[u][x] : -INFINITY;
-    }
-    float top = s[0][0];
+        for (int u = 0; u < PARTS; ++u)
+          s[u] = mma(row_frag<D>(kt, (u0 + u) * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
+      if (!full) {
+        asm volatile("");  // (a branch, not selects: most tiles need none)
+        const Seen mine = seen.from(u0 * 32 + h8);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < PARTS; ++u)
 #pragma unroll
-      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
-    top = fmaxf(top, other_half(top)) * c;
-    // (kept while no weight exceeds 2^8: the factor cancels in the end)
-    if (__any(top > m + 8.f)) {
-      const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
-      m = nm;
-      l *= by;
-#pragma unroll
-      for (int t2 = 0; t2 < D / 32; ++t2)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) acc[t2][x] *= by;
-    }
-    const float mm = m > -INFINITY ? m : 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
-        l += s[u][x];
+          for (int x = 0; x < 16; ++x) s[u][x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[u][x] : -INFINITY;
       }
-    add_rows<T, D>(acc, vt, 0, s[0]);
-    add_rows<T, D>(acc, vt, 32, s[1]);
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+      top = fmaxf(top, other_half(top)) * c;
+      // (kept while no weight exceeds 2^8: the factor cancels in the end)
+      if (__any(top > m + 8.f)) {
+        const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
+        m = nm;
+        l *= by;
+#pragma unroll
+        for (int t2 = 0; t2 < D / 32; ++t2)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[t2][x] *= by;
+      }
+      const float mm = m > -INFINITY ? m : 0.f;
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
+          l += s[u][x];
+        }
+#pragma unroll
+      for (int u = 0; u < PARTS; ++u) add_rows<T, D>(acc, vt, (u0 + u) * 32, s[u]);
+    }
   }
   l += other_half(l);
   // a row of no series gets zeros
@@ -321,10 +334,11 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
       ks.load(p.k, kv, tl.first(t + 1), false, tl.rows(t + 1));
       vs.load(p.v, kv, tl.first(t + 1), false, tl.rows(t + 1));
     }
-    if (j0 > r.wmax || !(j0 + WA_TILE > r.wlo || j0 < r.wstart + p.sinks)) continue;
+    if (!r.any(p, j0, WA_TILE)) continue;
     const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      if (!r.any(p, j0 + u * 32, 32)) continue;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int b = 0; b < D / 16; ++b) {
@@ -348,13 +362,10 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   store_own<T, D, VEC>(acc, p.scale, p.dq, rows_buffer<T>(p.dq, head, t0, own), r.i - t0);
 }
 
-// Last query row + 1 whose pairs with the key rows of tile [j0, j0 + WA_OWN) the main dk/dv kernel adds:
-// the window's, and the section's where the tile holds rows that stay visible.  Pairs of such a row
-// with later rows are the sink kernel's.
-__device__ inline int last_query(const WindowParams &p, int j0, bool sinks) {
-  int64_t hi = (int64_t)j0 + WA_OWN + p.window - 1;
-  const int64_t sec = ((int64_t)j0 / WA_SECTION + 1) * WA_SECTION;
-  if (sinks && sec > hi) hi = sec;
+// Last query row + 1 whose pairs with the key rows of tile [j0, j0 + WA_OWN) the main dk/dv kernel adds: the window's.
+// Pairs of rows that stay visible with later rows are the sink kernel's.
+__device__ inline int last_query(const WindowParams &p, int j0) {
+  const int64_t hi = (int64_t)j0 + WA_OWN + p.window - 1;
   return hi < p.s.n ? (int)hi : p.s.n;
 }
 
@@ -382,24 +393,21 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
     start = sp.start;
     end = (lane & 31) < p.sinks && j < sp.end ? sp.end : j;
     // a row of this kernel's tile of the other form has pairs up to last_query there
-    from = last_query(p, j / WA_OWN * WA_OWN, true);
+    from = last_query(p, j / WA_OWN * WA_OWN);
     i0 = sec0;
     i1 = sec0 + WA_SECTION < sp.end ? sec0 + WA_SECTION : sp.end;
     if (j / WA_SECTION >= tile) from = i1;  // (a sink row inside the section itself: all its pairs are the other form's)
   } else {
     const int j0 = tile * WA_OWN, j1 = j0 + WA_OWN < p.s.n ? j0 + WA_OWN : p.s.n;
     Offsets w = offsets_at(p.s, j0, false);
-    const Span first = span_of(p.s, w, j0, false);
     j = j0 + wave * 32 + (lane & 31);
     const Span mine = lane_span(p.s, w, j0, j1 - 1, j);
     const bool in = j < j1 && mine.start <= j;
     start = in ? mine.start : j;
     end = in ? mine.end : j;
     i0 = j0;
-    // every wave looks at the same rows: whether the tile holds rows that stay visible, and where the last series ends
     const Span last = span_of(p.s, w, j1 - 1, false);
-    const bool sinks = p.sinks > 0 && (first.end < j1 || (first.index >= 0 && first.start + p.sinks > j0));
-    i1 = last_query(p, j0, sinks);
+    i1 = last_query(p, j0);
     const int reach = last.index < 0 ? j1 : last.end;
     if (i1 > reach) i1 = reach;
     if (i1 < j1) i1 = j1;
@@ -433,7 +441,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   // of the wave: last series end, first query row of any, and what all have in common
   const int wend = wave_max(end), wfrom = SINK ? wave_max(from) : 0, wfirst = SINK ? wave_min(from) : 0;
   const int wlast = min_of(wave_min(end), i1);
-  const bool wall = __all(in);
+  const bool wall = __all(in), wsink = __any(in && j < start + p.sinks);
   for (int t = 0; t < count; ++t) {
     const int r0 = i0 + t % per_head * WA_TILE;
     __syncthreads();
@@ -466,7 +474,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
         if (wave != u || ru + 32 <= wfirst) continue;  // two waves share the section's rows
       } else {
         if (ru + 31 < wmin_j || ru >= wend) continue;
-        if (p.sinks == 0 && ru > wmax_j + p.window - 1) continue;
+        if (!wsink && ru > wmax_j + p.window - 1) continue;
       }
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
