@@ -31,16 +31,28 @@ struct WindowParams {
   float scale;
 };
 
-// Which streamed rows a lane's own row sees (or is seen by), as runs of the tile's rows: [lo, hi] of the window and
-// [slo, shi] of the rows that stay visible.
-struct Seen {
-  int lo, hi, slo, shi;
-  __device__ inline Seen from(int x) const { return {lo - x, hi - x, slo - x, shi - x}; }
-  __device__ inline bool operator()(int x) const { return ((x >= lo) & (x <= hi)) | ((x >= slo) & (x <= shi)); }
-};
 __device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ inline int min_of(int a, int b) { return a < b ? a : b; }
 __device__ inline int max_of(int a, int b) { return a > b ? a : b; }
+
+// Which rows of a streamed tile a lane's own row sees (or is seen by): the run [lo, hi], and [slo, shi] of the rows
+// that stay visible.
+struct Seen {
+  int lo, hi, slo, shi;
+  __device__ inline bool operator()(int x) const { return ((x >= lo) & (x <= hi)) | ((x >= slo) & (x <= shi)); }
+};
+// Weights (or scores) x of a part whose first row is `at` (of the tile, for the lane's half): `off` where not seen.
+template <bool SINKS> __device__ inline void mask_part(f32x16 &s, const Seen &seen, int at, float off) {
+  const int lo = seen.lo - at, n = max_of(seen.hi - seen.lo + 1, 0), slo = seen.slo - at, sn = max_of(seen.shi - seen.slo + 1, 0);
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const int r = 16 * (x >> 3) + (x & 7);
+    bool on = (uint32_t)(r - lo) < (uint32_t)n;
+    if (SINKS) on |= (uint32_t)(r - slo) < (uint32_t)sn;
+    s[x] = on ? s[x] : off;
+  }
+}
+
 
 // What a wave knows of its 32 own rows when they are query rows.
 struct QueryRows {
@@ -96,8 +108,8 @@ struct KeyTiles {
   }
 };
 
-// A tile with values that are not finite (rare) is cleaned before it is multiplied, since a masked row's weight of
-// zero would not keep them out; what the lane's own row sees of them is added here first.
+// A masked row's weight of zero does not keep a value that is not finite out of a product.  A tile that holds such
+// values (rare) is cleaned before it is multiplied, and what the lane's own row sees of them is added here first.
 // By element: as they are, for products whose weights are positive.
 template <typename T, int D, int NT> __device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
   const int h8 = (lane_id() >> 5) * 8;
@@ -146,6 +158,21 @@ __device__ inline void add_rows(f32x16 (&acc)[NT], const T *tile, int row0, cons
   }
 }
 
+// How the instructions up to here are to follow each other: LDS reads for AHEAD matrix instructions first, then one
+// matrix instruction, the reads (READS) of a later one and `valu` vector instructions in turn, so that neither the reads
+// nor the vector unit wait for the matrix core or it for them.
+template <int COUNT, int READS, int AHEAD, int VALU> __device__ inline void side_by_side() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i + AHEAD < COUNT) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if (VALU) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+  }
+}
+// Keeps the computation of a value from being moved behind this place.
+__device__ inline void hold(f32x16 &x) { asm volatile("" : "+v"(x)); }
+
 // The lane's own row, row `r` of the buffer.  Rows of no series (in = false) are zeros.
 template <typename T, int D, bool VEC>
 __device__ inline void load_own(Frag<T> (&f)[D / 16], const Rows &rows, Run buf, int r, bool in) {
@@ -169,7 +196,7 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
 }
 
 template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_forward_kernel(WindowParams p, int tiles) {
+__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2) void window_forward_kernel(WindowParams p, int tiles) {
   // float: matrix instructions are a sixteenth as fast, and parts that a wave does not see are left out one by one
   constexpr int PARTS = sizeof(T) == 4 ? 1 : 2;
   const int item = item_of_block(tiles * p.heads);
@@ -188,11 +215,13 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   Frag<T> qf[D / 16];
   load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
   f32x16 acc[D / 32];
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
-  float m = -INFINITY, l = 0.f;
+  float m, l;
   const float c = p.scale * kLog2e;
   Staged<T, D, WA_TILE, WA_THREADS, VEC> ks, vs;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
   ks.load(p.k, kv, tl.first(0), false, tl.rows(0));
   vs.load(p.v, kv, tl.first(0), false, tl.rows(0));
   for (int t = 0; t < tl.count; ++t) {
@@ -219,33 +248,27 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
     }
     if (!r.any(p, j0, WA_TILE)) continue;
     const bool full = r.all && j0 + WA_TILE - 1 <= r.wmin && j0 > r.wmax - p.window && j0 >= r.wstart;
-    // PARTS parts of 32 rows at a time
+    // Two parts of 32 rows.  The matrix cores work on one part's scores while the weights of the other are taken,
+    // and on the products with the first part's weights while those of the second are.
+    f32x16 s[2];
+    auto scores = [&](int u) __attribute__((always_inline)) {
+      s[u] = zero16();
 #pragma unroll
-    for (int u0 = 0; u0 < 2; u0 += PARTS) {
-      if (PARTS == 1 && !r.any(p, j0 + u0 * 32, 32)) continue;
-      f32x16 s[PARTS];
-#pragma unroll
-      for (int u = 0; u < PARTS; ++u) s[u] = zero16();
-#pragma unroll
-      for (int b = 0; b < D / 16; ++b)
-#pragma unroll
-        for (int u = 0; u < PARTS; ++u)
-          s[u] = mma(row_frag<D>(kt, (u0 + u) * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
+      for (int b = 0; b < D / 16; ++b) s[u] = mma(row_frag<D>(kt, u * 32 + pi_of(lane_id() & 31), 16 * b + h8), qf[b], s[u]);
+    };
+    auto mask = [&](int u) __attribute__((always_inline)) {
       if (!full) {
         asm volatile("");  // (a branch, not selects: most tiles need none)
-        const Seen mine = seen.from(u0 * 32 + h8);
-#pragma unroll
-        for (int u = 0; u < PARTS; ++u)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) s[u][x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[u][x] : -INFINITY;
+        if (j0 < r.wstart + p.sinks) mask_part<true>(s[u], seen, u * 32 + h8, -INFINITY);
+        else mask_part<false>(s[u], seen, u * 32 + h8, -INFINITY);
       }
-      float top = s[0][0];
+    };
+    // A new maximum is taken only when some weight would exceed 2^8: the factor cancels in the end.
+    auto maximum = [&](const f32x16 &of, bool behind) __attribute__((always_inline)) {
+      float top = of[0];
 #pragma unroll
-      for (int u = 0; u < PARTS; ++u)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) top = fmaxf(top, s[u][x]);
+      for (int x = 1; x < 16; ++x) top = fmaxf(top, of[x]);
       top = fmaxf(top, other_half(top)) * c;
-      // (kept while no weight exceeds 2^8: the factor cancels in the end)
       if (__any(top > m + 8.f)) {
         const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
         m = nm;
@@ -254,17 +277,61 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
         for (int t2 = 0; t2 < D / 32; ++t2)
 #pragma unroll
           for (int x = 0; x < 16; ++x) acc[t2][x] *= by;
+        if (behind)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) s[0][x] *= by;  // (weights by now)
       }
+    };
+    auto weights = [&](int u) __attribute__((always_inline)) {
       const float mm = m > -INFINITY ? m : 0.f;
 #pragma unroll
-      for (int u = 0; u < PARTS; ++u)
+      for (int x = 0; x < 16; ++x) {
+        s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
+        l += s[u][x];
+      }
+    };
+    if (PARTS == 1) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s[u][x] = exp2_hw(__builtin_fmaf(s[u][x], c, -mm));
-          l += s[u][x];
-        }
+      for (int u = 0; u < 2; ++u) {
+        if (!r.any(p, j0 + u * 32, 32)) continue;
+        scores(u);
+        mask(u);
+        maximum(s[u], false);
+        weights(u);
+        add_rows<T, D>(acc, vt, u * 32, s[u]);
+      }
+    } else if (D == 128) {
+      constexpr int N = D / 16, VALU = 64 / N;
+      scores(0);
+      side_by_side<N, 1, 4, 0>();
+      mask(0);
+      maximum(s[0], false);
+      weights(0);
+      scores(1);
+      side_by_side<N, 1, 4, VALU>();
+      hold(s[0]);
+      mask(1);
+      maximum(s[1], true);
+      add_rows<T, D>(acc, vt, 0, s[0]);
+      weights(1);
+      side_by_side<N, 2, 3, VALU>();
+      hold(s[1]);
+      add_rows<T, D>(acc, vt, 32, s[1]);
+      side_by_side<N, 2, 3, 0>();
+    } else {
+      // (three waves a SIMD fit: they fill each other's waits, and one maximum serves both parts)
+      scores(0);
+      scores(1);
+      mask(0);
+      mask(1);
+      f32x16 both;
 #pragma unroll
-      for (int u = 0; u < PARTS; ++u) add_rows<T, D>(acc, vt, (u0 + u) * 32, s[u]);
+      for (int x = 0; x < 16; ++x) both[x] = fmaxf(s[0][x], s[1][x]);
+      maximum(both, false);
+      weights(0);
+      weights(1);
+      add_rows<T, D>(acc, vt, 0, s[0]);
+      add_rows<T, D>(acc, vt, 32, s[1]);
     }
   }
   l += other_half(l);
@@ -306,10 +373,10 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
   const float lse2 = in ? p.lse[(int64_t)r.i * p.heads + head] * kLog2e : 0.f;
   f32x16 acc[D / 32];
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
   const float c = p.scale * kLog2e;
   Staged<T, D, WA_TILE, WA_THREADS, VEC> ks, vs;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) acc[t] = zero16();
   ks.load(p.k, kv, tl.first(0), false, tl.rows(0));
   vs.load(p.v, kv, tl.first(0), false, tl.rows(0));
   for (int t = 0; t < tl.count; ++t) {
@@ -352,9 +419,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
       }
       if (!full) {
         asm volatile("");
-        const Seen mine = seen.from(h8);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] = mine(u * 32 + 16 * (x >> 3) + (x & 7)) ? s[x] : 0.f;
+        if (j0 < r.wstart + p.sinks) mask_part<true>(s, seen, u * 32 + h8, 0.f);
+        else mask_part<false>(s, seen, u * 32 + h8, 0.f);
       }
       add_rows<T, D>(acc, kt, u * 32, s);
     }
@@ -419,13 +485,11 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   load_own<T, D, VEC>(kf, p.k, rows_buffer<T>(p.k, kv, j_first, own), j - j_first, in);
   load_own<T, D, VEC>(vf, p.v, rows_buffer<T>(p.v, kv, j_first, own), j - j_first, in);
   f32x16 dk[D / 32], dv[D / 32];
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t) { dk[t] = zero16(); dv[t] = zero16(); }
   const float c = p.scale * kLog2e;
   const int per_head = (i1 - i0 + WA_TILE - 1) / WA_TILE, count = per_head * group;
   Staged<T, D, WA_TILE, WA_THREADS, VEC> qs, ds;
   float lse_n = 0.f, delta_n = 0.f;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t) __attribute__((always_inline)) {
     const int head = kv * group + t / per_head, first = i0 + t % per_head * WA_TILE;
     const int rows = i1 - first < WA_TILE ? i1 - first : WA_TILE;
     qs.load(p.q, head, first, false, rows);
@@ -436,12 +500,14 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
       delta_n = p.delta[at];
     }
   };
-  if (count > 0) fetch(0);
   const int wmin_j = SINK ? start : tile * WA_OWN + wave * 32, wmax_j = wmin_j + 31;
   // of the wave: last series end, first query row of any, and what all have in common
   const int wend = wave_max(end), wfrom = SINK ? wave_max(from) : 0, wfirst = SINK ? wave_min(from) : 0;
   const int wlast = min_of(wave_min(end), i1);
   const bool wall = __all(in), wsink = __any(in && j < start + p.sinks);
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) { dk[t] = zero16(); dv[t] = zero16(); }
+  if (count > 0) fetch(0);
   for (int t = 0; t < count; ++t) {
     const int r0 = i0 + t % per_head * WA_TILE;
     __syncthreads();
@@ -490,14 +556,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
       }
       if (!(wall && ru >= wmax_j && ru >= wfrom && ru + 31 < wlast && ru + 31 < wmin_j + p.window)) {
         asm volatile("");
-        const Seen mine = seen.from(h8);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int row = u * 32 + 16 * (x >> 3) + (x & 7);
-          const bool on = (row >= mine.lo) & (row <= mine.hi);
-          s[x] = on ? s[x] : 0.f;
-          dp[x] = on ? dp[x] : 0.f;
-        }
+        mask_part<false>(s, seen, u * 32 + h8, 0.f);
+        mask_part<false>(dp, seen, u * 32 + h8, 0.f);
       }
       add_rows<T, D>(dv, dt, u * 32, s);
       add_rows<T, D>(dk, qt, u * 32, dp);
