@@ -23,7 +23,8 @@
 
 namespace tmp {
 
-constexpr int DA_PIECE = 64;
+// Rows that travel to LDS together: as many as leave the state its registers.
+constexpr int da_piece(int dk) { return dk == 128 ? 32 : 64; }
 
 struct DecayParams {
   Series s;
@@ -115,15 +116,20 @@ template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 3
   for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, k0, 32 * t), v, st[t]);
 }
 
+// Waves a SIMD: two where state, tiles on their way and decays fit 256 registers without spilling.
+constexpr int da_waves(int bytes, int dk, int dv, bool out) {
+  return (dk == 128 && (out || bytes == 4)) || (bytes == 4 && dk == 64 && out) || dv < dk ? 1 : 2;
+}
+
 // OUT: walks a section and writes its rows.  Otherwise: walks the rows of the section that belong to the
 // series which goes on behind it, and leaves the state that they make in carry[section + 1].
 //
 // A wave owns 32 columns of the values and that strip of the state, in registers; the queries', keys' and
 // values' tiles of 64 rows are shared, the next ones on their way meanwhile.  Rows are worked on in parts of
 // SUB, whose decays are the same for every part (held in registers) but a series' last one.
-template <typename T, int D, bool VEC, bool OUT, bool EXACT>
-__global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2) void decay_walk_kernel(DecayParams p) {
-  constexpr int NT = D / 32, THREADS = D * 2, SUB = 32;
+template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
+__global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void decay_walk_kernel(DecayParams p) {
+  constexpr int NT = DK / 32, THREADS = DV * 2, SUB = 32, DA_PIECE = da_piece(DK);
   const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
   const int kd = p.k.dim, vd = p.v.dim;
@@ -144,7 +150,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
     sp = walk_span(p, near, sec0);
   }
   extern __shared__ __align__(16) unsigned char smem[];
-  T *kt = (T *)smem, *vt = kt + DA_PIECE * D, *qt = vt + DA_PIECE * D;
+  T *kt = (T *)smem, *vt = kt + DA_PIECE * DK, *qt = vt + DA_PIECE * DV;
   __shared__ int flag[2];
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   const float ld = p.log_decay[head] * kLog2e;
@@ -164,7 +170,8 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
 #pragma unroll
   for (int t = 0; t < NT; ++t) st[t] = zero16();
   bool fresh = true;
-  Staged<T, D, DA_PIECE, THREADS, VEC, true> qs, ks, vs;
+  Staged<T, DK, DA_PIECE, THREADS, VEC, true> qs, ks;
+  Staged<T, DV, DA_PIECE, THREADS, VEC, true> vs;
   auto fetch = [&](int at, int len) {
     const int64_t first = p.reverse ? (int64_t)p.s.n - 1 - at : at;
     ks.load(p.k, head, first, p.reverse, len);
@@ -193,7 +200,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
     if (__builtin_expect(dirty, 0)) {
 #pragma unroll 1
       for (int j = 0; j < DA_PIECE; ++j) {
-        const bool on = !finite(tile_elem<T, D>(vt, j, strip + pi_of(l31)));
+        const bool on = !finite(tile_elem<T, DV>(vt, j, strip + pi_of(l31)));
         if (j < 32) bad[0] = on && j < bad[0] ? j : bad[0];
         else bad[1] = on && j - 32 < bad[1] ? j - 32 : bad[1];
       }
@@ -229,9 +236,9 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
       if (OUT) {
         f32x16 acc = zero16(), s = zero16();
 #pragma unroll
-        for (int b = 0; b < D / 16; ++b) {
-          const Frag<T> qf = row_frag<D>(qt, r0 + l31, 16 * b + h8);
-          s = mma(row_frag<D>(kt, r0 + pi_of(l31), 16 * b + h8), qf, s);
+        for (int b = 0; b < DK / 16; ++b) {
+          const Frag<T> qf = row_frag<DK>(qt, r0 + l31, 16 * b + h8);
+          s = mma(row_frag<DK>(kt, r0 + pi_of(l31), 16 * b + h8), qf, s);
           acc = mma(operand<T>(st[b >> 1], b & 1), qf, acc);
         }
 #pragma unroll
@@ -240,7 +247,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
           s[x] = 16 * (x >> 3) + h8 + (x & 7) <= l31 ? s[x] * wd[x] : 0.f;
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc = mma(col_frag<D>(vt, r0 + 16 * b, strip), operand<T>(s, b), acc);
+        for (int b = 0; b < 2; ++b) acc = mma(col_frag<DV>(vt, r0 + 16 * b, strip), operand<T>(s, b), acc);
         if (__builtin_expect(dirty, 0)) {  // they reach the rows at and behind their own, as NaN
           const int first = r0 ? bad[1] : bad[0];
 #pragma unroll
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
       if (rows == SUB) {
 #pragma unroll
         for (int b = 0; b < SUB / 16; ++b)
-          state_add<D, EXACT>(st, kt, r0 + 16 * b, w_all + 8 * b, col_frag<D>(vt, r0 + 16 * b, strip));
+          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w_all + 8 * b, col_frag<DV>(vt, r0 + 16 * b, strip));
       } else {
 #pragma unroll 1
         for (int b = 0; 16 * b < rows; ++b) {
@@ -274,7 +281,7 @@ __global__ __launch_bounds__(D * 2, D == 128 && (OUT || sizeof(T) == 4) ? 1 : 2)
             const int left = rows - 1 - (16 * b + h8 + e);
             w[e] = left >= 0 ? power(ld, left + post) : 0.f;
           }
-          state_add<D, EXACT>(st, kt, r0 + 16 * b, w, col_frag<D>(vt, r0 + 16 * b, strip));
+          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip));
         }
       }
       if (__builtin_expect(dirty, 0)) {
@@ -307,7 +314,7 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int64_t 
   float *c = p.carry + (int64_t)head * per_head + e;
   const int64_t step = (int64_t)p.heads * per_head;
   float x = 0.f;
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 32;
   for (int s = 1; s < p.sections; s += AHEAD) {
     float add[AHEAD];
     int link[AHEAD];
@@ -346,8 +353,8 @@ __global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t
 static int decay_section(int64_t n, int heads) {
   int64_t s = (n * heads + 1023) / 1024;
   if (s > n) s = n;
-  s = (s + DA_PIECE - 1) / DA_PIECE * DA_PIECE;
-  if (s < DA_PIECE) s = DA_PIECE;
+  s = (s + 63) / 64 * 64;
+  if (s < 64) s = 64;
   return (int)s;
 }
 
@@ -381,30 +388,52 @@ static int decay_check(const tmp_decay_attention_args *a, const char *what, bool
   return TMP_OK;
 }
 
-template <typename T, int D, bool VEC, bool EXACT> static void decay_walk(const DecayParams &p, hipStream_t st) {
-  const int threads = D * 2, piece = DA_PIECE * D * (int)sizeof(T);
+template <typename T, int DK, int DV, bool VEC, bool EXACT> static void decay_walk(const DecayParams &p, hipStream_t st) {
+  const int threads = DV * 2, row = da_piece(DK) * (int)sizeof(T);
   if (p.sections > 1) {
     {
       ProfScope ps("decay_walk_kernel(states)", st);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, VEC, false, EXACT>), dim3((p.sections - 1) * p.heads),
-                         dim3(threads), 2 * piece, st, p);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, false, EXACT>), dim3((p.sections - 1) * p.heads),
+                         dim3(threads), row * (DK + DV), st, p);
     }
     const int64_t per_head = (int64_t)p.k.dim * p.v.dim;
     TMP_LAUNCH(decay_scan_kernel, dim3((unsigned)((per_head + 255) / 256 * p.heads)), dim3(256), st, p, per_head);
   }
   ProfScope ps("decay_walk_kernel", st);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, D, VEC, true, EXACT>), dim3(p.sections * p.heads), dim3(threads),
-                     3 * piece, st, p);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, true, EXACT>), dim3(p.sections * p.heads), dim3(threads),
+                     row * (2 * DK + DV), st, p);
 }
-template <typename T, int D, bool VEC> static void decay_walk_form(const DecayParams &p, hipStream_t st) {
-  if (sizeof(T) == 2 && p.state_out) decay_walk<T, D, VEC, sizeof(T) == 2>(p, st);
-  else decay_walk<T, D, VEC, false>(p, st);
-}
-
-static void decay_run(const DecayParams &p, int type, hipStream_t st) {
-  const int d = padded_dim(p.k.dim > p.v.dim ? p.k.dim : p.v.dim);
+template <typename T, int DK, int DV> static void decay_walk_form(const DecayParams &p, hipStream_t st) {
   const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec;
-  TMP_BY_FORM(decay_walk_form, type, d, vec, p, st);
+  constexpr bool SPLIT = sizeof(T) == 2;
+  if (SPLIT && p.state_out) {
+    if (vec) decay_walk<T, DK, DV, true, SPLIT>(p, st);
+    else decay_walk<T, DK, DV, false, SPLIT>(p, st);
+  } else {
+    if (vec) decay_walk<T, DK, DV, true, false>(p, st);
+    else decay_walk<T, DK, DV, false, false>(p, st);
+  }
+}
+// Both head sizes padded to 32, 64 or 128, and at most a factor of two apart.
+template <typename T> static void decay_walk_dims(const DecayParams &p, hipStream_t st) {
+  int dk = padded_dim(p.k.dim), dv = padded_dim(p.v.dim);
+  if (dk < dv / 2) dk = dv / 2;
+  if (dv < dk / 2) dv = dk / 2;
+  if (dk == 32) {
+    if (dv == 32) decay_walk_form<T, 32, 32>(p, st);
+    else decay_walk_form<T, 32, 64>(p, st);
+  } else if (dk == 64) {
+    if (dv == 32) decay_walk_form<T, 64, 32>(p, st);
+    else if (dv == 64) decay_walk_form<T, 64, 64>(p, st);
+    else decay_walk_form<T, 64, 128>(p, st);
+  } else {
+    if (dv == 64) decay_walk_form<T, 128, 64>(p, st);
+    else decay_walk_form<T, 128, 128>(p, st);
+  }
+}
+static void decay_run(const DecayParams &p, int type, hipStream_t st) {
+  if (type == TMP_F32) decay_walk_dims<float>(p, st);
+  else decay_walk_dims<__bf16>(p, st);
 }
 
 static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d) {
