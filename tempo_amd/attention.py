@@ -37,11 +37,13 @@ def _on_device(t, name, device=None):
 
 
 def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
-    """[rows, heads, dim], innermost dimension contiguous; type and device of `like`."""
+    """[rows, heads, dim], innermost dimension contiguous; type and device of `like`.  Returns the rows to hand on: a copy
+    where they overlap in memory (a broadcast row) or lie 2^22 elements or more apart."""
     if like is not None and isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.device == like.device and t.dim() == 3:
-        have, last = t.shape, t.stride()[2]  # the usual case, asked for at once: small calls are bound by their host part
+        # the usual case, asked for at once: small calls are bound by their host part
+        have, (row, _, last) = t.shape, t.stride()
         if have[0] == n and (heads is None or have[1] == heads) and (dim is None or have[2] == dim) and last == 1:
-            if have[1] and have[2]:
+            if have[1] and have[2] and (n <= 1 or have[2] <= row < 2 ** 22):
                 return t
     _on_device(t, name, None if like is None else like.device)
     if t.dtype not in _TYPES:
@@ -57,7 +59,7 @@ def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
         raise ValueError(f"{name} needs at least one head and one element")
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name} must be contiguous in its innermost dimension")
-    return t
+    return t if t.shape[0] <= 1 or t.shape[2] <= t.stride(0) < 2 ** 22 else t.contiguous()
 
 
 def _plain_check(t, name, dtype, shape, device):
@@ -125,10 +127,10 @@ def series_offsets(key, n_keys):
 # ---- linear attention with a decay for each head -------------------------------------------------
 
 def _decay_args(q, k, v, log_decay, offsets, scale, state):
-    _rows_check(q, "q")
+    q = _rows_check(q, "q")
     n, heads, dk = q.shape
-    _rows_check(k, "k", q, n, heads, dk)
-    _rows_check(v, "v", q, n, heads)
+    k = _rows_check(k, "k", q, n, heads, dk)
+    v = _rows_check(v, "v", q, n, heads)
     dv = v.shape[2]
     _plain_check(log_decay, "log_decay", torch.float32, (heads,), q.device)
     if log_decay.requires_grad:
@@ -139,6 +141,7 @@ def _decay_args(q, k, v, log_decay, offsets, scale, state):
     a = DecayAttentionArgs(n=n, n_series=n_series, offsets=_p(offsets), type=_TYPES[q.dtype], heads=heads, dim_k=dk,
                            dim_v=dv, scale=_scale(scale, dk), log_decay=log_decay.data_ptr(), q=_ref(q), k=_ref(k),
                            v=_ref(v), state_in=_p(state))
+    a.held = (q, k, v)  # (copies live as long as the pointers to them)
     return a, n_series
 
 
@@ -165,7 +168,7 @@ def decay_attention_grad(dout, q, k, v, log_decay, offsets=None, scale=None, sta
     a, n_series = _decay_args(q, k, v, log_decay, offsets, scale, state)
     n, heads, dk = q.shape
     dv = v.shape[2]
-    _rows_check(dout, "dout", q, n, heads, dv)
+    dout = _rows_check(dout, "dout", q, n, heads, dv)
     if dstate is not None:
         _plain_check(dstate, "dstate", torch.float32, (n_series, heads, dk, dv), q.device)
     gq, gk = (torch.empty((n, heads, dk), dtype=q.dtype, device=q.device) for _ in range(2))
@@ -230,10 +233,10 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One new row for each of some series: q, k [b, heads, dk], v [b, heads, dv]; state float32 [n_slots, heads,
     dk, dv], changed in place; slots int32 [b] (None: row i is slot i).  A row whose slot is out of range or named
     by an earlier row changes nothing and results in NaN.  Returns out [b, heads, dv]."""
-    _rows_check(q, "q")
+    q = _rows_check(q, "q")
     n, heads, dk = q.shape
-    _rows_check(k, "k", q, n, heads, dk)
-    _rows_check(v, "v", q, n, heads)
+    k = _rows_check(k, "k", q, n, heads, dk)
+    v = _rows_check(v, "v", q, n, heads)
     dv = v.shape[2]
     _plain_check(log_decay, "log_decay", torch.float32, (heads,), q.device)
     _on_device(state, "state", q.device)
@@ -254,17 +257,19 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
 # ---- attention over a sliding window -------------------------------------------------------------
 
 def _window_args(q, k, v, window, sinks, offsets, scale):
-    _rows_check(q, "q")
+    q = _rows_check(q, "q")
     n, heads, dk = q.shape
-    _rows_check(k, "k", q, n, None, dk)
+    k = _rows_check(k, "k", q, n, None, dk)
     kv = k.shape[1]
-    _rows_check(v, "v", q, n, kv)
+    v = _rows_check(v, "v", q, n, kv)
     if heads % kv:
         raise ValueError(f"{heads} query heads cannot share {kv} key/value heads")
     n_series = _offsets_check(offsets, q.device)
-    return WindowAttentionArgs(n=n, n_series=n_series, offsets=_p(offsets), type=_TYPES[q.dtype], heads=heads, kv_heads=kv,
-                               dim_k=dk, dim_v=v.shape[2], window=min(_int_arg(window, "window", 1), 2 ** 62),
-                               sinks=_int_arg(sinks, "sinks", 0), scale=_scale(scale, dk), q=_ref(q), k=_ref(k), v=_ref(v))
+    a = WindowAttentionArgs(n=n, n_series=n_series, offsets=_p(offsets), type=_TYPES[q.dtype], heads=heads, kv_heads=kv,
+                            dim_k=dk, dim_v=v.shape[2], window=min(_int_arg(window, "window", 1), 2 ** 62),
+                            sinks=_int_arg(sinks, "sinks", 0), scale=_scale(scale, dk), q=_ref(q), k=_ref(k), v=_ref(v))
+    a.held = (q, k, v)
+    return a
 
 
 def _window_forward(q, k, v, window, sinks, offsets, scale, return_lse):
@@ -281,8 +286,8 @@ def window_attention_grad(dout, q, k, v, out, lse, window, sinks=0, offsets=None
     """Backward of `window_attention`: (dq, dk, dv) from dout and what the forward returned (out, lse)."""
     a = _window_args(q, k, v, window, sinks, offsets, scale)
     n, heads, dv = q.shape[0], q.shape[1], v.shape[2]
-    _rows_check(dout, "dout", q, n, heads, dv)
-    _rows_check(out, "out", q, n, heads, dv)
+    dout = _rows_check(dout, "dout", q, n, heads, dv)
+    out = _rows_check(out, "out", q, n, heads, dv)
     _plain_check(lse, "lse", torch.float32, (n, heads), q.device)
     gq, gk, gv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
     a.out, a.lse, a.dout, a.dq, a.dk, a.dv = _ref(out), lse.data_ptr(), _ref(dout), _ref(gq), _ref(gk), _ref(gv)
@@ -354,9 +359,9 @@ def window_cache_write(k, v, k_cache, v_cache, length, sinks=0, offsets=None, sl
     """Fills cache slots from whole series: after `window_attention` over k, v [n, kv_heads, dim], slot slots[s] (None:
     s) holds what `window_attention_step` needs of series s, in place of what it held.  k_cache, v_cache [n_slots,
     window + sinks, kv_heads, dim]; length int64 [n_slots]: rows seen by each slot."""
-    _rows_check(k, "k")
+    k = _rows_check(k, "k")
     n, kv, dk = k.shape
-    _rows_check(v, "v", k, n, kv)
+    v = _rows_check(v, "v", k, n, kv)
     dv = v.shape[2]
     n_series = _offsets_check(offsets, k.device)
     n_slots, window, sinks = _caches_check(k_cache, v_cache, length, sinks, k, kv, dk, dv)
@@ -374,11 +379,11 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
     it) and attends with q [b, heads, dk] over the slot's last `window` rows, the new one included, and its first
     `sinks`.  The caches' number of rows is window + sinks.  slots int32 [b] (None: row i is slot i); a row whose slot is
     out of range or named by an earlier row changes nothing and results in NaN.  Returns out [b, heads, dv]."""
-    _rows_check(q, "q")
+    q = _rows_check(q, "q")
     n, heads, dk = q.shape
-    _rows_check(k, "k", q, n, None, dk)
+    k = _rows_check(k, "k", q, n, None, dk)
     kv = k.shape[1]
-    _rows_check(v, "v", q, n, kv)
+    v = _rows_check(v, "v", q, n, kv)
     dv = v.shape[2]
     if heads % kv:
         raise ValueError(f"{heads} query heads cannot share {kv} key/value heads")

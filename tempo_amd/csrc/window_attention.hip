@@ -270,8 +270,10 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T
       for (int x = 1; x < 16; ++x) top = fmaxf(top, of[x]);
       top = fmaxf(top, other_half(top)) * c;
       if (__any(top > m + 8.f)) {
-        const float nm = fmaxf(m, top), by = nm > -INFINITY ? exp2_hw(m - nm) : 1.f;
-        m = nm;
+        // (each row by itself: what other rows of the wave hold does not show in its rounding)
+        const bool up = top > m + 8.f;
+        const float by = up ? exp2_hw(m - top) : 1.f;
+        m = up ? top : m;
         l *= by;
 #pragma unroll
         for (int t2 = 0; t2 < D / 32; ++t2)
