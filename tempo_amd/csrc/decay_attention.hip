@@ -24,7 +24,7 @@
 namespace tmp {
 
 // Rows that travel to LDS together: as many as leave the state its registers.
-constexpr int da_piece(int dk) { return dk == 128 ? 32 : 64; }
+constexpr int da_piece(int bytes, int dk) { return dk * bytes >= 256 ? 32 : 64; }
 
 struct DecayParams {
   Series s;
@@ -119,7 +119,7 @@ template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 3
 
 // Waves a SIMD: two where state, tiles on their way and decays fit 256 registers without spilling.
 constexpr int da_waves(int bytes, int dk, int dv, bool out) {
-  return (dk == 128 && (out || bytes == 4)) || (bytes == 4 && dk == 64 && out) || dv < dk ? 1 : 2;
+  return (dk == 128 && (out || bytes == 4)) || dv < dk ? 1 : 2;
 }
 
 // OUT: walks a section and writes its rows.  Otherwise: walks the rows of the section that belong to the
@@ -130,7 +130,7 @@ constexpr int da_waves(int bytes, int dk, int dv, bool out) {
 // SUB, whose decays are the same for every part (held in registers) but a series' last one.
 template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
 __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void decay_walk_kernel(DecayParams p) {
-  constexpr int NT = DK / 32, THREADS = DV * 2, SUB = 32, DA_PIECE = da_piece(DK);
+  constexpr int NT = DK / 32, THREADS = DV * 2, SUB = 32, DA_PIECE = da_piece(sizeof(T), DK);
   const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
   const int kd = p.k.dim, vd = p.v.dim;
@@ -240,6 +240,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
         f32x16 acc = zero16(), s = zero16();
 #pragma unroll
         for (int b = 0; b < DK / 16; ++b) {
+          if (sizeof(T) == 4 && 16 * b >= kd) break;  // (float's instructions are long enough to be worth the branch)
           const Frag<T> qf = row_frag<DK>(qt, r0 + l31, 16 * b + h8);
           s = mma(row_frag<DK>(kt, r0 + pi_of(l31), 16 * b + h8), qf, s);
           acc = mma(operand<T>(st[b >> 1], b & 1), qf, acc);
@@ -397,7 +398,7 @@ static int decay_check(const tmp_decay_attention_args *a, const char *what, bool
 }
 
 template <typename T, int DK, int DV, bool VEC, bool EXACT> static void decay_walk(const DecayParams &p, hipStream_t st) {
-  const int threads = DV * 2, row = da_piece(DK) * (int)sizeof(T);
+  const int threads = DV * 2, row = da_piece(sizeof(T), DK) * (int)sizeof(T);
   if (p.sections > 1 && !p.alone) {
     {
       ProfScope ps("decay_walk_kernel(states)", st);
