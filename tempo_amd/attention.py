@@ -39,11 +39,13 @@ def _on_device(t, name, device=None):
 def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
     """[rows, heads, dim], innermost dimension contiguous; type and device of `like`.  Returns the rows to hand on: a copy
     where they overlap in memory (a broadcast row) or lie 2^22 elements or more apart."""
-    if like is not None and isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.device == like.device and t.dim() == 3:
+    if isinstance(t, torch.Tensor) and t.dim() == 3 and t.is_cuda and t.dtype in _TYPES:
         # the usual case, asked for at once: small calls are bound by their host part
-        have, (row, _, last) = t.shape, t.stride()
-        if have[0] == n and (heads is None or have[1] == heads) and (dim is None or have[2] == dim) and last == 1:
-            if have[1] and have[2] and (n <= 1 or have[2] <= row < 2 ** 22):
+        (rows, h, d), (row, _, last) = t.shape, t.stride()
+        if last == 1 and h and d and (rows <= 1 or d <= row < 2 ** 22):
+            if like is None:
+                return t
+            if rows == n and heads in (None, h) and dim in (None, d) and t.dtype is like.dtype and t.device == like.device:
                 return t
     _on_device(t, name, None if like is None else like.device)
     if t.dtype not in _TYPES:
@@ -66,8 +68,8 @@ def _plain_check(t, name, dtype, shape, device):
     _on_device(t, name, device)
     if t.dtype != dtype:
         raise TypeError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t
@@ -153,7 +155,7 @@ def _decay_call(fn, a, device):
 
 def _decay_forward(q, k, v, log_decay, offsets, scale, state, return_state):
     a, n_series = _decay_args(q, k, v, log_decay, offsets, scale, state)
-    out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=q.dtype, device=q.device)
+    out = q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
     last = None
     if return_state:
         last = torch.empty((n_series, q.shape[1], q.shape[2], v.shape[2]), dtype=torch.float32, device=q.device)
@@ -222,11 +224,10 @@ def _slots_check(slots, n, n_slots, device):
     _plain_check(slots, "slots", torch.int32, (n,), device)
 
 
-def _no_grad(**tensors):
-    for name, t in tensors.items():
-        if t.requires_grad:
-            if torch.is_grad_enabled():
-                raise ValueError(f"{name} requires a gradient; a step has none (use the form over whole series)")
+def _no_grad(*tensors):
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("an argument requires a gradient; a step has none (use the form over whole series)")
 
 
 def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
@@ -244,8 +245,8 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
         raise ValueError("state must be [n_slots, heads, dk, dv]")
     _plain_check(state, "state", torch.float32, (state.shape[0], heads, dk, dv), q.device)
     _slots_check(slots, n, state.shape[0], q.device)
-    _no_grad(q=q, k=k, v=v, state=state, log_decay=log_decay)
-    out = torch.empty((n, heads, dv), dtype=q.dtype, device=q.device)
+    _no_grad(q, k, v, state, log_decay)
+    out = q.new_empty((n, heads, dv))
     a = DecayAttentionStepArgs(n=n, n_slots=state.shape[0], slots=_p(slots), type=_TYPES[q.dtype], heads=heads, dim_k=dk,
                                dim_v=dv, scale=_scale(scale, dk), log_decay=log_decay.data_ptr(), q=_ref(q), k=_ref(k),
                                v=_ref(v), out=_ref(out), state=state.data_ptr())
@@ -274,7 +275,7 @@ def _window_args(q, k, v, window, sinks, offsets, scale):
 
 def _window_forward(q, k, v, window, sinks, offsets, scale, return_lse):
     a = _window_args(q, k, v, window, sinks, offsets, scale)
-    out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=q.dtype, device=q.device)
+    out = q.new_empty((q.shape[0], q.shape[1], v.shape[2]))
     lse = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device) if return_lse else None
     a.out, a.lse = _ref(out), _p(lse)
     with _current(q.device):
@@ -330,7 +331,7 @@ def window_attention(q, k, v, window, sinks=0, offsets=None, scale=None, return_
 
 
 def _caches_check(k_cache, v_cache, length, sinks, like, kv_heads, dk, dv):
-    """(n_slots, window) of a pair of caches [n_slots, window + sinks, kv_heads, dim]."""
+    """(n_slots, window, sinks) of a pair of caches [n_slots, window + sinks, kv_heads, dim]."""
     for t, name, dim in ((k_cache, "k_cache", dk), (v_cache, "v_cache", dv)):
         _on_device(t, name, like.device)
         if t.dtype != like.dtype:
@@ -339,7 +340,7 @@ def _caches_check(k_cache, v_cache, length, sinks, like, kv_heads, dk, dv):
             raise ValueError(f"{name} must be [n_slots, window + sinks, {kv_heads}, {dim}], got {tuple(t.shape)}")
         if dim > 1 and t.stride(3) != 1:
             raise ValueError(f"{name} must be contiguous in its innermost dimension")
-        if any(t.shape[i] > 1 and t.stride(i) == 0 for i in range(3)):
+        if 0 in t.stride() and any(t.shape[i] > 1 and t.stride(i) == 0 for i in range(3)):
             raise ValueError(f"{name} must not repeat its rows (expanded tensor)")
     if k_cache.shape[:2] != v_cache.shape[:2]:
         raise ValueError("k_cache and v_cache must have the same slots and rows")
@@ -366,7 +367,7 @@ def window_cache_write(k, v, k_cache, v_cache, length, sinks=0, offsets=None, sl
     n_series = _offsets_check(offsets, k.device)
     n_slots, window, sinks = _caches_check(k_cache, v_cache, length, sinks, k, kv, dk, dv)
     _slots_check(slots, n_series, n_slots, k.device)
-    _no_grad(k_cache=k_cache, v_cache=v_cache)
+    _no_grad(k_cache, v_cache)
     a = WindowCacheWriteArgs(n=n, n_series=n_series, offsets=_p(offsets), n_slots=n_slots, slots=_p(slots),
                              type=_TYPES[k.dtype], kv_heads=kv, dim_k=dk, dim_v=dv, window=window, sinks=sinks, k=_ref(k),
                              v=_ref(v), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache), length=length.data_ptr())
@@ -389,8 +390,8 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
         raise ValueError(f"{heads} query heads cannot share {kv} key/value heads")
     n_slots, window, sinks = _caches_check(k_cache, v_cache, length, sinks, q, kv, dk, dv)
     _slots_check(slots, n, n_slots, q.device)
-    _no_grad(q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
-    out = torch.empty((n, heads, dv), dtype=q.dtype, device=q.device)
+    _no_grad(q, k, v, k_cache, v_cache)
+    out = q.new_empty((n, heads, dv))
     a = WindowAttentionStepArgs(n=n, n_slots=n_slots, slots=_p(slots), type=_TYPES[q.dtype], heads=heads, kv_heads=kv,
                                 dim_k=dk, dim_v=dv, window=window, sinks=sinks, scale=_scale(scale, dk), q=_ref(q), k=_ref(k),
                                 v=_ref(v), out=_ref(out), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache),
