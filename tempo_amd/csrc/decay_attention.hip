@@ -283,7 +283,9 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
         const Run o = rows_buffer<T>(p.out, head, p.reverse ? (int64_t)p.s.n - r - rows : r, pos < sec0 ? 0 : rows);
         const uint32_t at = (uint32_t)((p.reverse ? rows - 1 - l31 : l31) * (int)p.out.row * (int)sizeof(T));
 #pragma unroll
-        for (int b = 0; b < 2; ++b) buffer_store8(o, at, strip + 16 * b + h8, p.out.dim, VEC, operand<T>(acc, b));
+        for (int b = 0; b < 2; ++b)
+          // (backwards, rows from `rows` on would start below zero: they have no elements)
+          buffer_store8(o, at, strip + 16 * b + h8, VEC || l31 < rows ? p.out.dim : 0, VEC, operand<T>(acc, b));
       }
       if (sp.index < 0 || (ends && r0 + SUB >= len && !p.state_out)) continue;  // no state, or nobody reads it
       const float fade = rows == SUB ? fade_all : power(ld, rows);

@@ -52,6 +52,8 @@ WINDOW = [
     ("long", 0, 0, 2, 2, 16, 100, 600, 1),
     ("long", 200, 200, 1, 1, 32, 32, 7, 7),
     ("many", 5, 5, 2, 1, 72, 72, 20, 3),
+    ("many", 5, 6, 1, 1, 85, 9, 20, 3),
+    ("long", 1, 0, 3, 1, 7, 121, 50, 2),
 ]
 
 
@@ -87,6 +89,10 @@ DECAY = [
     ("long", 0, 0, 2, 40, 72, [-0.1, -1e-4], True),
     ("long", 200, 200, 1, 100, 16, [-0.05], True),
     ("many", 5, 5, 2, 24, 24, [-0.22314355, -0.01], True),
+    # odd sizes of one head: rows that start at odd multiples of two bytes
+    ("many", 5, 6, 1, 85, 9, [-0.1], False),
+    ("long", 1, 0, 1, 85, 9, [-0.1], True),
+    ("many", 0, 0, 3, 7, 121, [-0.1, -0.5, -0.01], True),
 ]
 
 
