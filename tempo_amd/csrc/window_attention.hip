@@ -21,6 +21,10 @@ constexpr int WA_TILE = 64;    // rows of a streamed tile
 constexpr int WA_THREADS = 256;
 constexpr int WA_SECTION = WA_OWN;  // query rows whose share of the sinks' gradients one block adds up
 
+// Up to this window dS enters its products as two bfloat16 numbers: with few rows the error of do.o (of the rounded out)
+// is large beside dS, and a second rounding would show (error against 64 bits at window 11: 2.6e-3 with one number).
+constexpr int WA_FINE = 64;
+
 struct WindowParams {
   Series s;
   Rows q, k, v, out, dout, dq, dk, dv;
@@ -172,6 +176,17 @@ template <int COUNT, int READS, int AHEAD, int VALU> __device__ inline void side
 }
 // Keeps the computation of a value from being moved behind this place.
 __device__ inline void hold(f32x16 &x) { asm volatile("" : "+v"(x)); }
+
+// What rounding a part's weights to the operand's type leaves of them.
+template <typename T> __device__ inline f32x16 left_over(f32x16 w) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const Frag<T> f = operand<T>(w, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[8 * b + e] -= (float)f[e];
+  }
+  return w;
+}
 
 // The lane's own row, row `r` of the buffer.  Rows of no series (in = false) are zeros.
 template <typename T, int D, bool VEC>
@@ -425,6 +440,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
         else mask_part<false>(s, seen, u * 32 + h8, 0.f);
       }
       add_rows<T, D>(acc, kt, u * 32, s);
+      if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(acc, kt, u * 32, left_over<T>(s));
     }
   }
   store_own<T, D, VEC>(acc, p.scale, p.dq, rows_buffer<T>(p.dq, head, t0, own), r.i - t0);
@@ -563,6 +579,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
       }
       add_rows<T, D>(dv, dt, u * 32, s);
       add_rows<T, D>(dk, qt, u * 32, dp);
+      if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(dk, qt, u * 32, left_over<T>(dp));
     }
   }
   if (SINK) {
