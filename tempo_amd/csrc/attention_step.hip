@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) >= 512 ? 1 : 2) void window_step
   Staged<T, D, 32, 64, VEC> vs;
   auto fetch = [&](int row0) {
     const int rows = r1 - row0 < 32 ? r1 - row0 : 32;
-    const Run kb = rows_buffer<T>(kc, kv, row0, rows);
+    const Run kb = rows_buffer<T, !VEC>(kc, kv, row0, rows);  // (what rows behind the last read is masked below)
     const uint32_t at = pi_of(l31) * (uint32_t)kc.row * (uint32_t)sizeof(T);
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) kf[x] = buffer_load8<T>(kb, at, 16 * x + h8, kc.dim, VEC);
@@ -171,6 +171,7 @@ __global__ __launch_bounds__(256, D * sizeof(T) >= 512 ? 1 : 2) void window_step
     f32x16 s = zero16();
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) s = mma(kf[x], qf[x], s);
+    vs.settle();
     vs.store(vt);
     if (row0 + 32 < r1) fetch(row0 + 32);
     __builtin_amdgcn_wave_barrier();

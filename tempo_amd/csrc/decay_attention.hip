@@ -208,9 +208,12 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
   fetch(pos, sp.index < 0 ? 0 : len);
   while (true) {
     __syncthreads();
+    ks.settle();
+    vs.settle();
     ks.store(kt);
     vs.store(vt);
     if (OUT) {
+      qs.settle();
       qs.store(qt);
       if (vs.dirty()) flag[turn] = 1;
     }
@@ -285,7 +288,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
 #pragma unroll
         for (int b = 0; b < 2; ++b)
           // (backwards, rows from `rows` on would start below zero: they have no elements)
-          buffer_store8(o, at, strip + 16 * b + h8, VEC || l31 < rows ? p.out.dim : 0, VEC, operand<T>(acc, b));
+          buffer_store8<T>(o, at, strip + 16 * b + h8, VEC || l31 < rows ? p.out.dim : 0, VEC, operand<T>(acc, b));
       }
       if (sp.index < 0 || (ends && r0 + SUB >= len && !p.state_out)) continue;  // no state, or nobody reads it
       const float fade = rows == SUB ? fade_all : power(ld, rows);

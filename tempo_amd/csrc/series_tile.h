@@ -110,7 +110,7 @@ template <typename F> __device__ inline F cleaned(F f) {
 // (pointer and strides multiples of 16 bytes, dim a multiple of eight elements), decided by the host;
 // kernels come in two forms, VEC for calls whose every array allows them.
 //
-// A run of rows is accessed through a buffer descriptor that ends behind its last row: what lies outside
+// A run of rows is accessed through a buffer descriptor that ends behind its last row's last element: what lies outside
 // reads as zero and is not written, so that odd lengths and head sizes cost no branch.
 struct Rows {
   void *p;
@@ -132,78 +132,79 @@ struct Run {
   Buffer b;
   uint32_t lead;
 };
-template <typename T> __device__ inline Run rows_buffer(const Rows &r, int head, int64_t first, int count) {
+//
+// For reading, the end is moved up to a multiple of four bytes: element loads are made of whole words.  An allocation
+// holds every word that it holds a byte of; what such a word has of others is masked.
+template <typename T, bool READ = false> __device__ inline Run rows_buffer(const Rows &r, int head, int64_t first, int count) {
   // (the same for all lanes of a wave: said to the compiler, which would loop over the lanes' values otherwise)
   const uint64_t at = (uint64_t)(head_of<T>(r, head) + first * r.row);
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
-  const uint32_t bytes = (uint32_t)count * (uint32_t)r.row * (uint32_t)sizeof(T), lead = lo & 3;
+  const uint32_t lead = lo & 3;
+  uint32_t bytes = count > 0 ? ((uint32_t)(count - 1) * (uint32_t)r.row + (uint32_t)r.dim) * (uint32_t)sizeof(T) + lead : 0;
+  if (READ) bytes = (bytes + 3) & ~3u;
   Run run;
-  run.b = buffer_of((void *)(((uint64_t)hi << 32) | (lo & ~3u)), __builtin_amdgcn_readfirstlane(bytes) + lead);
+  run.b = buffer_of((void *)(((uint64_t)hi << 32) | (lo & ~3u)), __builtin_amdgcn_readfirstlane(bytes));
   run.lead = lead;
   return run;
 }
 constexpr uint32_t kOutside = 0xfffffff0u;  // a byte offset behind every buffer's end
 
-// Eight elements from d on of the row that starts `at` bytes into the buffer, zeros beyond dim.
-template <typename T> __device__ inline Frag<T> buffer_load8(Run u, uint32_t at, int d, int dim, bool vec);
-template <> __device__ inline bf16x8 buffer_load8<__bf16>(Run u, uint32_t at, int d, int dim, bool vec) {
-  const Buffer b = u.b;
-  if (vec) return __builtin_bit_cast(bf16x8, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, d < dim ? at + d * 2 : kOutside, 0, 0));
-  bf16x8 f;
+// Eight elements from d on of the row that starts `at` bytes into the buffer.  Words of a buffer may lie at any
+// multiple of four bytes, so only two things keep rows of other sizes from being read like VEC's: bfloat16 at an odd
+// place, for which a fifth word is read and the words are shifted, and what lies behind the row's end, which is
+// masked.  settled() does both once the words are there (2739 rows x 12 x 77: forward 67 us with single loads, 39 us so).
+template <typename T> __device__ inline void buffer_words8(Run u, uint32_t at, int d, int dim, bool vec, Frag<T> *f, uint32_t *fifth) {
+  const uint32_t o = d < dim ? (vec ? at : u.lead + at) + d * (uint32_t)sizeof(T) : kOutside;
+  if (sizeof(T) == 2) {
+    const uint32_t w = o & ~3u;  // (outside stays outside)
+    const u32x4 x = (u32x4)__builtin_amdgcn_raw_buffer_load_b128(u.b, vec ? o : w, 0, 0);
+    __builtin_memcpy(f, &x, 16);
+    if (!vec) *fifth = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(u.b, d < dim ? w + 16 : kOutside, 0, 0);
+  } else {
+    const u32x4 x = (u32x4)__builtin_amdgcn_raw_buffer_load_b128(u.b, o, 0, 0);
+    const u32x4 y = (u32x4)__builtin_amdgcn_raw_buffer_load_b128(u.b, d < dim ? o + 16 : kOutside, 0, 0);
+    __builtin_memcpy(f, &x, 16);
+    __builtin_memcpy((char *)f + 16, &y, 16);
+  }
+}
+// `left`: elements of the row from d on; `odd`: bytes that the first one lies behind its word's start.
+__device__ inline bf16x8 settled(bf16x8 f, uint32_t fifth, uint32_t odd, int left) {
+  u32x4 x = __builtin_bit_cast(u32x4, f);
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    f[e] = __builtin_bit_cast(__bf16, __builtin_amdgcn_raw_buffer_load_b16(b, d + e < dim ? u.lead + at + (d + e) * 2 : kOutside, 0, 0));
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t to = c < 3 ? x[c < 3 ? c + 1 : 3] : fifth;
+    x[c] = __builtin_amdgcn_alignbyte(to, x[c], odd) & (left > 2 * c + 1 ? ~0u : left > 2 * c ? 0xffffu : 0u);
+  }
+  return __builtin_bit_cast(bf16x8, x);
+}
+__device__ inline f32x8 settled(f32x8 f, uint32_t, uint32_t, int left) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = e < left ? f[e] : 0.f;
   return f;
 }
-template <> __device__ inline f32x8 buffer_load8<float>(Run u, uint32_t at, int d, int dim, bool vec) {
-  const Buffer b = u.b;
-  f32x8 f;
-  if (vec) {
-    const uint32_t o = d < dim ? at + d * 4 : kOutside;
-    const f32x4 x = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, o, 0, 0));
-    const f32x4 y = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(b, d < dim ? o + 16 : kOutside, 0, 0));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { f[e] = x[e]; f[e + 4] = y[e]; }
-    return f;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    f[e] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, d + e < dim ? at + (d + e) * 4 : kOutside, 0, 0));
-  return f;
+template <typename T> __device__ inline Frag<T> buffer_load8(Run u, uint32_t at, int d, int dim, bool vec) {
+  Frag<T> f;
+  uint32_t fifth = 0;
+  buffer_words8<T>(u, at, d, dim, vec, &f, &fifth);
+  return vec ? f : settled(f, fifth, (u.lead + at) & 3, dim - d);
 }
-__device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, bf16x8 f) {
-  const Buffer b = u.b;
-  if (vec) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), b, d < dim ? at + d * 2 : kOutside, 0, 0);
-    return;
-  }
+
+// Whole pieces at a word's start in one or two stores; the others element by element.
+template <typename T> __device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, Frag<T> f) {
+  const uint32_t o = (vec ? at : u.lead + at) + d * (uint32_t)sizeof(T);
+  const bool whole = vec ? d < dim : d + 8 <= dim && (o & 3) == 0;
+  u32x4 w[sizeof(T) / 2];
+  __builtin_memcpy(w, &f, sizeof(f));
+#pragma unroll
+  for (int c = 0; c < (int)sizeof(T) / 2; ++c) __builtin_amdgcn_raw_buffer_store_b128(w[c], u.b, whole ? o + 16 * c : kOutside, 0, 0);
+  if (vec || whole || d >= dim) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const __bf16 x = f[e];
-    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x), b, d + e < dim ? u.lead + at + (d + e) * 2 : kOutside, 0, 0);
+    const T x = f[e];
+    const uint32_t to = d + e < dim ? o + e * (uint32_t)sizeof(T) : kOutside;
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x), u.b, to, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), u.b, to, 0, 0);
   }
-}
-__device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, f32x8 f) {
-  const Buffer b = u.b;
-  if (vec) {
-    f32x4 x, y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { x[e] = f[e]; y[e] = f[e + 4]; }
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), b, d < dim ? at + d * 4 : kOutside, 0, 0);
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), b, d < dim ? at + d * 4 + 16 : kOutside, 0, 0);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = f[e];
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), b, d + e < dim ? at + (d + e) * 4 : kOutside, 0, 0);
-  }
-}
-template <typename F> __device__ inline F zero_frag() {
-  F f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = 0;
-  return f;
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------
@@ -274,11 +275,15 @@ template <typename T, int D, int ROWS, int THREADS, bool VEC, bool FRESH = false
   static constexpr int kCount = ROWS * kPerRow / THREADS;
   static_assert(ROWS * kPerRow % THREADS == 0 && THREADS % kPerRow == 0, "whole pieces");
   static constexpr int kStep = THREADS / kPerRow;  // rows from one of a thread's pieces to its next
+  static_assert(kStep % 2 == 0, "all of a thread's rows start at odd places or none");
+  static constexpr bool kFifth = !VEC && sizeof(T) == 2;
   Frag<T> f[kCount];
+  uint32_t fifth[kFifth ? kCount : 1], odd;
+  int left;
   // rows first + r, or with `back` first - r, for r in [0, count) are read, the others become zeros
   __device__ inline void load(const Rows &rows, int head, int64_t first, bool back, int count) {
     const int tid = threadIdx.x % THREADS, r0 = tid / kPerRow, d = (tid % kPerRow) * 8;
-    const Run b = rows_buffer<T>(rows, head, back ? first - (count - 1) : first, count);
+    const Run b = rows_buffer<T, !VEC>(rows, head, back ? first - (count - 1) : first, count);
     const int row = (int)rows.row * (int)sizeof(T);
     // (backwards, rows from `count` on lie before the buffer: offsets below zero, which are outside too)
     int at = back ? (count - 1 - r0) * row : r0 * row;
@@ -286,10 +291,17 @@ template <typename T, int D, int ROWS, int THREADS, bool VEC, bool FRESH = false
     if (FRESH) asm volatile("" : "+v"(at));  // (the pieces' offsets are worked out anew each time: cheaper than registers)
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
-      int from = at + i * step;
-      if (!VEC) asm volatile("" : "+v"(from));  // (offsets of single elements are not worth registers)
-      f[i] = buffer_load8<T>(b, from, d, VEC || r0 + i * kStep < count ? rows.dim : 0, VEC);
+      const int dim = VEC || r0 + i * kStep < count ? rows.dim : 0;
+      buffer_words8<T>(b, at + i * step, d, dim, VEC, &f[i], &fifth[kFifth ? i : 0]);
     }
+    odd = (b.lead + at) & 3;
+    left = rows.dim - d;
+  }
+  // the words into elements, before they are looked at or stored
+  __device__ inline void settle() {
+    if (VEC) return;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) f[i] = settled(f[i], fifth[kFifth ? i : 0], odd, left);
   }
   __device__ inline void store(T *t) const {
     const int tid = threadIdx.x % THREADS, r0 = tid / kPerRow, d = (tid % kPerRow) * 8;

@@ -206,7 +206,7 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
 #pragma unroll
     for (int x = 0; x < 16; ++x) c[x] *= by;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) buffer_store8(buf, at, t * 32 + 16 * b + h8, rows.dim, VEC, operand<T>(c, b));
+    for (int b = 0; b < 2; ++b) buffer_store8<T>(buf, at, t * 32 + 16 * b + h8, rows.dim, VEC, operand<T>(c, b));
   }
 }
 
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T
   const bool in = r.start <= r.i;
   const int own = p.s.n - t0 < WA_OWN ? p.s.n - t0 : WA_OWN;
   Frag<T> qf[D / 16];
-  load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
+  load_own<T, D, VEC>(qf, p.q, rows_buffer<T, !VEC>(p.q, head, t0, own), r.i - t0, in);
   f32x16 acc[D / 32];
   float m, l;
   const float c = p.scale * kLog2e;
@@ -242,6 +242,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T
   for (int t = 0; t < tl.count; ++t) {
     const int j0 = tl.first(t), j1 = tl.end(t);
     __syncthreads();
+    ks.settle();
+    vs.settle();
     ks.store(kt);
     vs.store(vt);
     if (vs.dirty()) flag[t & 1] = 1;
@@ -376,8 +378,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   const bool in = r.start <= r.i;
   const int own = p.s.n - t0 < WA_OWN ? p.s.n - t0 : WA_OWN;
   Frag<T> qf[D / 16], of[D / 16];
-  load_own<T, D, VEC>(of, p.out, rows_buffer<T>(p.out, head, t0, own), r.i - t0, in);
-  load_own<T, D, VEC>(qf, p.dout, rows_buffer<T>(p.dout, head, t0, own), r.i - t0, in);
+  load_own<T, D, VEC>(of, p.out, rows_buffer<T, !VEC>(p.out, head, t0, own), r.i - t0, in);
+  load_own<T, D, VEC>(qf, p.dout, rows_buffer<T, !VEC>(p.dout, head, t0, own), r.i - t0, in);
   float delta = 0.f;
 #pragma unroll
   for (int b = 0; b < D / 16; ++b)
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   if (r.i < p.s.n && lane_id() < 32) p.delta[(int64_t)r.i * p.heads + head] = delta;
 #pragma unroll
   for (int b = 0; b < D / 16; ++b) of[b] = qf[b];
-  load_own<T, D, VEC>(qf, p.q, rows_buffer<T>(p.q, head, t0, own), r.i - t0, in);
+  load_own<T, D, VEC>(qf, p.q, rows_buffer<T, !VEC>(p.q, head, t0, own), r.i - t0, in);
   const float lse2 = in ? p.lse[(int64_t)r.i * p.heads + head] * kLog2e : 0.f;
   f32x16 acc[D / 32];
   const float c = p.scale * kLog2e;
@@ -399,6 +401,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
   for (int t = 0; t < tl.count; ++t) {
     const int j0 = tl.first(t), j1 = tl.end(t);
     __syncthreads();
+    ks.settle();
+    vs.settle();
     ks.store(kt);
     vs.store(vt);
     if (ks.dirty()) flag[t & 1] = 1;
@@ -500,8 +504,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   Frag<T> kf[D / 16], vf[D / 16];
   // the block's own rows, from j_first on (a series' first rows may be fewer than 32)
   const int j_first = SINK ? start : tile * WA_OWN, own = p.s.n - j_first < WA_OWN ? p.s.n - j_first : WA_OWN;
-  load_own<T, D, VEC>(kf, p.k, rows_buffer<T>(p.k, kv, j_first, own), j - j_first, in);
-  load_own<T, D, VEC>(vf, p.v, rows_buffer<T>(p.v, kv, j_first, own), j - j_first, in);
+  load_own<T, D, VEC>(kf, p.k, rows_buffer<T, !VEC>(p.k, kv, j_first, own), j - j_first, in);
+  load_own<T, D, VEC>(vf, p.v, rows_buffer<T, !VEC>(p.v, kv, j_first, own), j - j_first, in);
   f32x16 dk[D / 32], dv[D / 32];
   const float c = p.scale * kLog2e;
   const int per_head = (i1 - i0 + WA_TILE - 1) / WA_TILE, count = per_head * group;
@@ -529,6 +533,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   for (int t = 0; t < count; ++t) {
     const int r0 = i0 + t % per_head * WA_TILE;
     __syncthreads();
+    qs.settle();
+    ds.settle();
     qs.store(qt);
     ds.store(dt);
     if (qs.dirty() || ds.dirty()) flag[t & 1] = 1;
