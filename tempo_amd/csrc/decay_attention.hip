@@ -258,7 +258,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
 #pragma unroll 1
     for (int r0 = 0; r0 < len; r0 += SUB) {
       const int rows = len - r0 < SUB ? len - r0 : SUB;
-      if (OUT) {
+      if (OUT && pos >= sec0) {
         f32x16 acc = zero16(), s = zero16();
 #pragma unroll
         for (int b = 0; b < DK / 16; ++b) {
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
           }
         }
         const int r = pos + r0;
-        const Run o = rows_buffer<T>(p.out, head, p.reverse ? (int64_t)p.s.n - r - rows : r, pos < sec0 ? 0 : rows);
+        const Run o = rows_buffer<T>(p.out, head, p.reverse ? (int64_t)p.s.n - r - rows : r, rows);
         const uint32_t at = (uint32_t)((p.reverse ? rows - 1 - l31 : l31) * (int)p.out.row * (int)sizeof(T));
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -400,12 +400,15 @@ __global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// Sections of whole pieces, as few as give the 1024 SIMDs two waves each (a block has one for 32 of dv): every one
-// more adds a state to be written, strung together and read.  131072 x 16 x 128 bf16: 512 blocks 913 us, 1024 955 us,
-// 2048 1017 us; 50000 x 16 x 64: a walk takes 113 us with 1024 or 2048 blocks, 120 us with 512.
-static int decay_section(int64_t n, int heads, int dim) {
-  const int dv = padded_dim(dim);  // the larger of the two sizes: either is the values' in some walk
-  const int blocks = 2048 / (dv / 32);
+// Sections of whole pieces, as few as give the 1024 SIMDs the two waves each that they hold (a block has one for 32 of
+// dv): every one more adds a state to be written, strung together and read.  131072 x 16 x 128 bf16: 512 blocks 913 us,
+// 1024 955 us, 2048 1017 us; 50000 x 16 x 64: a walk takes 113 us with 1024 or 2048 blocks, 120 us with 512.  Float
+// with both sizes above 64 has one wave a SIMD: 14350 x 3 x 116/71 training 603 us with 512 blocks, 465 us with 256
+// (and 30011 x 8 x 40/72, two waves: 237 us with 512, 283 us with 256).
+static int decay_section(int64_t n, int heads, int dim_k, int dim_v, int bytes) {
+  const int dk = padded_dim(dim_k), dv = padded_dim(dim_v);
+  const int least = dk < dv ? dk : dv, most = dk < dv ? dv : dk;  // (either is the values' in some walk)
+  const int blocks = (bytes == 4 && least == 128 ? 1024 : 2048) / (most / 32);
   int64_t s = (n * heads + blocks - 1) / blocks;
   if (s > n) s = n;
   s = (s + 63) / 64 * 64;
@@ -420,7 +423,7 @@ struct DecayPlan {
 };
 static void decay_plan(const tmp_decay_attention_args *a, Workspace &ws, DecayPlan *d) {
   const int64_t n = a->n > 0 ? a->n : 1;
-  d->section = decay_section(n, a->heads, a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
+  d->section = decay_section(n, a->heads, a->dim_k, a->dim_v, a->type == TMP_F32 ? 4 : 2);
   d->sections = (int)((n + d->section - 1) / d->section);
   d->carry = ws.take<float>((size_t)d->sections * a->heads * a->dim_k * a->dim_v);
   d->link = ws.take<int32_t>(d->sections + 1);
