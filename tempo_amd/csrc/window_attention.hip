@@ -115,10 +115,10 @@ struct KeyTiles {
 // A masked row's weight of zero does not keep a value that is not finite out of a product.  A tile that holds such
 // values (rare) is cleaned before it is multiplied, and what the lane's own row sees of them is added here first.
 // By element: as they are, for products whose weights are positive.
-template <typename T, int D, int NT> __device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
+template <typename T, int D, int ROWS = WA_TILE, int NT> __device__ inline void add_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
   const int h8 = (lane_id() >> 5) * 8;
 #pragma unroll 1
-  for (int j = 0; j < WA_TILE; ++j) {
+  for (int j = 0; j < ROWS; ++j) {
     const bool on = seen(j);
     int row = j;
     asm volatile("" : "+v"(row));  // keeps the addresses below out of the registers of the main path
@@ -133,10 +133,10 @@ template <typename T, int D, int NT> __device__ inline void add_not_finite(f32x1
   }
 }
 // By row: NaN for every element, where the weight itself depends on such a value.
-template <typename T, int D, int NT> __device__ inline void mark_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
+template <typename T, int D, int ROWS = WA_TILE, int NT> __device__ inline void mark_not_finite(f32x16 (&acc)[NT], const T *tile, Seen seen) {
   bool bad = false;
 #pragma unroll 1
-  for (int j = 0; j < WA_TILE; ++j) {
+  for (int j = 0; j < ROWS; ++j) {
     bool any = false;
     for (int d = lane_id(); d < D; d += 64) any |= !finite(tile_elem<T, D>(tile, j, d));
     bad |= __any(any) & seen(j);
@@ -159,6 +159,17 @@ __device__ inline void add_rows(f32x16 (&acc)[NT], const T *tile, int row0, cons
       const Frag<T> f = col_frag<D>(tile, row0 + 16 * b, t * 32);
       acc[t] = mma(f, wf, acc[t]);
     }
+  }
+}
+
+// The same with the lane's number given, for places that are to be worked out anew.
+template <int D, int NT>
+__device__ inline void add_rows_at(f32x16 (&acc)[NT], const float *tile, int row0, const f32x16 &w, int l) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const f32x8 wf = operand<float>(w, b);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = mma(col_frag<D>(tile, row0 + 16 * b, t * 32, l), wf, acc[t]);
   }
 }
 
@@ -462,13 +473,17 @@ __device__ inline int last_query(const WindowParams &p, int j0) {
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
 template <typename T, int D, bool VEC, bool SINK>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
+  // Float of 128: the own rows and both sums take 256 of the 512 registers.  Tiles of 32 rows, whose places in LDS are
+  // worked out anew for each, leave enough of the others (7950 x 28 x 128, window 94: 1103 us otherwise, 650 us so).
+  constexpr bool TIGHT = D * sizeof(T) >= 512 && !SINK;
+  constexpr int TILE = TIGHT ? 32 : WA_TILE;
   const int item = item_of_block(tiles * p.kv_heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
   const int kv = item / tiles, tile = item % tiles;
   const int wave = wave_id(), lane = lane_id(), h8 = (lane >> 5) * 8;
-  __shared__ __align__(16) T qt[WA_TILE * D], dt[WA_TILE * D];
-  __shared__ float lse_t[WA_TILE], delta_t[WA_TILE];
+  __shared__ __align__(16) T qt[TILE * D], dt[TILE * D];
+  __shared__ float lse_t[TILE], delta_t[TILE];
   __shared__ int flag[2];
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   int j, start, end, i0, i1, from = 0;  // the lane's key row and its series; query rows [i0, i1), those before `from` left out
@@ -508,15 +523,15 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   load_own<T, D, VEC>(vf, p.v, rows_buffer<T, !VEC>(p.v, kv, j_first, own), j - j_first, in);
   f32x16 dk[D / 32], dv[D / 32];
   const float c = p.scale * kLog2e;
-  const int per_head = (i1 - i0 + WA_TILE - 1) / WA_TILE, count = per_head * group;
-  Staged<T, D, WA_TILE, WA_THREADS, VEC> qs, ds;
+  const int per_head = (i1 - i0 + TILE - 1) / TILE, count = per_head * group;
+  Staged<T, D, TILE, WA_THREADS, VEC> qs, ds;
   float lse_n = 0.f, delta_n = 0.f;
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int head = kv * group + t / per_head, first = i0 + t % per_head * WA_TILE;
-    const int rows = i1 - first < WA_TILE ? i1 - first : WA_TILE;
+    const int head = kv * group + t / per_head, first = i0 + t % per_head * TILE;
+    const int rows = i1 - first < TILE ? i1 - first : TILE;
     qs.load(p.q, head, first, false, rows);
     ds.load(p.dout, head, first, false, rows);
-    if (threadIdx.x < WA_TILE && (int)threadIdx.x < rows) {
+    if (threadIdx.x < TILE && (int)threadIdx.x < rows) {
       const int64_t at = (int64_t)(first + threadIdx.x) * p.heads + head;
       lse_n = p.lse[at] * kLog2e;
       delta_n = p.delta[at];
@@ -531,7 +546,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
   for (int t = 0; t < D / 32; ++t) { dk[t] = zero16(); dv[t] = zero16(); }
   if (count > 0) fetch(0);
   for (int t = 0; t < count; ++t) {
-    const int r0 = i0 + t % per_head * WA_TILE;
+    const int r0 = i0 + t % per_head * TILE;
     __syncthreads();
     qs.settle();
     ds.settle();
@@ -539,15 +554,15 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
     ds.store(dt);
     if (qs.dirty() || ds.dirty()) flag[t & 1] = 1;
     if (threadIdx.x == 0) flag[(t & 1) ^ 1] = 0;
-    if (threadIdx.x < WA_TILE) { lse_t[threadIdx.x] = lse_n; delta_t[threadIdx.x] = delta_n; }
+    if (threadIdx.x < TILE) { lse_t[threadIdx.x] = lse_n; delta_t[threadIdx.x] = delta_n; }
     __syncthreads();
     // query rows [first, last] of a tile see key row j: those of its window, all behind it if it stays visible
     const int last = min_of(end, i1) - 1 - r0;
     const Seen seen = {max_of(j, from) - r0, min_of(j < start + p.sinks ? last : j + p.window - 1 - r0, last), 0, -1};
     if (__builtin_expect(flag[t & 1], 0)) {
       if (!SINK || wave == 0) {  // (two waves share a section's rows: the first speaks for both)
-        add_not_finite<T, D>(dv, dt, seen);
-        mark_not_finite<T, D>(dk, qt, seen);
+        add_not_finite<T, D, TILE>(dv, dt, seen);
+        mark_not_finite<T, D, TILE>(dk, qt, seen);
       }
       __syncthreads();
       qs.clean();
@@ -558,19 +573,22 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
     }
     if (t + 1 < count) fetch(t + 1);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < TILE / 32; ++u) {
       const int ru = r0 + u * 32;
       if (SINK) {
-        if (wave != u || ru + 32 <= wfirst) continue;  // two waves share the section's rows
+        if (wave != (ru - i0) / 32 % 2 || ru + 32 <= wfirst) continue;  // two waves share the section's rows
       } else {
         if (ru + 31 < wmin_j || ru >= wend) continue;
         if (!wsink && ru > wmax_j + p.window - 1) continue;
       }
+      int l = lane;
+      if (TIGHT) asm volatile("" : "+v"(l));
+      const int h = TIGHT ? (l >> 5) * 8 : h8;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int b = 0; b < D / 16; ++b) {
-        s = mma(row_frag<D>(qt, u * 32 + pi_of(lane & 31), 16 * b + h8), kf[b], s);
-        dp = mma(row_frag<D>(dt, u * 32 + pi_of(lane & 31), 16 * b + h8), vf[b], dp);
+        s = mma(row_frag<D>(qt, u * 32 + pi_of(l & 31), 16 * b + h), kf[b], s);
+        dp = mma(row_frag<D>(dt, u * 32 + pi_of(l & 31), 16 * b + h), vf[b], dp);
       }
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
@@ -583,9 +601,14 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
         mask_part<false>(s, seen, u * 32 + h8, 0.f);
         mask_part<false>(dp, seen, u * 32 + h8, 0.f);
       }
-      add_rows<T, D>(dv, dt, u * 32, s);
-      add_rows<T, D>(dk, qt, u * 32, dp);
-      if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(dk, qt, u * 32, left_over<T>(dp));
+      if constexpr (TIGHT) {
+        add_rows_at<D>(dv, dt, u * 32, s, l);
+        add_rows_at<D>(dk, qt, u * 32, dp, l);
+      } else {
+        add_rows<T, D>(dv, dt, u * 32, s);
+        add_rows<T, D>(dk, qt, u * 32, dp);
+        if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(dk, qt, u * 32, left_over<T>(dp));
+      }
     }
   }
   if (SINK) {
