@@ -793,6 +793,7 @@ typedef struct {
   float *dstate_in;
 } tmp_decay_attention_args;
 
+/* Of the call that takes these args: the backward one, which needs more, has dout.p set. */
 size_t tmp_decay_attention_workspace_bytes(const tmp_decay_attention_args *a);
 int tmp_decay_attention(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream);
 int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void *workspace, size_t workspace_bytes, void *stream);

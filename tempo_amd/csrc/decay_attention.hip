@@ -40,6 +40,11 @@ struct DecayParams {
   float scale, in_by, out_by;   // of rows, and of states read and written
 };
 
+// Walks that are launched together, one to each blockIdx.y: the backward pass's three have the same sections.
+struct DecayWalks {
+  DecayParams p[3];
+};
+
 // lambda^m with m >= 0; lambda may be 0 (log2 = -infinity).
 __device__ inline float power(float log2_decay, int m) { return m == 0 ? 1.f : exp2_hw(log2_decay * (float)m); }
 
@@ -129,7 +134,8 @@ constexpr int da_waves(int bytes, int dk, int dv, bool out) {
 // values' tiles of 64 rows are shared, the next ones on their way meanwhile.  Rows are worked on in parts of
 // SUB, whose decays are the same for every part (held in registers) but a series' last one.
 template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
-__global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void decay_walk_kernel(DecayParams p) {
+__global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void decay_walk_kernel(DecayWalks w) {
+  const DecayParams &p = w.p[blockIdx.y];
   constexpr int NT = DK / 32, THREADS = DV * 2, SUB = 32, DA_PIECE = da_piece(sizeof(T), DK);
   const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
@@ -340,7 +346,8 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
 // elements together, x -> m x + y, the waves of a block theirs through LDS: one trip to memory in place of one
 // for every run of sections (64074 rows x 4 x 12, 501 sections: 22 us, 58 us by one wave).
 constexpr int DA_RUN = 16, DA_SCAN_WAVES = 16;
-__global__ __launch_bounds__(DA_SCAN_WAVES * 64) void decay_scan_kernel(DecayParams p, int64_t per_head) {
+__global__ __launch_bounds__(DA_SCAN_WAVES * 64) void decay_scan_kernel(DecayWalks walks, int64_t per_head) {
+  const DecayParams &p = walks.p[blockIdx.y];
   const int64_t blocks = (per_head + 63) / 64;
   const int head = (int)(blockIdx.x / blocks), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -420,13 +427,15 @@ struct DecayPlan {
   float *carry;
   int32_t *link;
   int section, sections;
+  size_t per_walk;  // floats of carry
 };
-static void decay_plan(const tmp_decay_attention_args *a, Workspace &ws, DecayPlan *d) {
+static void decay_plan(const tmp_decay_attention_args *a, int walks, Workspace &ws, DecayPlan *d) {
   const int64_t n = a->n > 0 ? a->n : 1;
   d->section = decay_section(n, a->heads, a->dim_k, a->dim_v, a->type == TMP_F32 ? 4 : 2);
   d->sections = (int)((n + d->section - 1) / d->section);
-  d->carry = ws.take<float>((size_t)d->sections * a->heads * a->dim_k * a->dim_v);
-  d->link = ws.take<int32_t>(d->sections + 1);
+  d->per_walk = (size_t)d->sections * a->heads * a->dim_k * a->dim_v;
+  d->carry = ws.take<float>(d->per_walk * walks);
+  d->link = ws.take<int32_t>((size_t)(d->sections + 1) * walks);
 }
 
 static int decay_check(const tmp_decay_attention_args *a, const char *what, bool grad) {
@@ -446,62 +455,66 @@ static int decay_check(const tmp_decay_attention_args *a, const char *what, bool
   return TMP_OK;
 }
 
-template <typename T, int DK, int DV, bool VEC, bool EXACT> static void decay_walk(const DecayParams &p, hipStream_t st) {
+template <typename T, int DK, int DV, bool VEC, bool EXACT> static void decay_walk(const DecayWalks &w, int walks, hipStream_t st) {
+  const DecayParams &p = w.p[0];
   const int threads = DV * 2, row = da_piece(sizeof(T), DK) * (int)sizeof(T);
   if (p.sections > 1 && !p.alone) {
     {
       ProfScope ps("decay_walk_kernel(states)", st);
-      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, false, EXACT>), dim3((p.sections - 1) * p.heads),
-                         dim3(threads), row * (DK + DV), st, p);
+      hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, false, EXACT>), dim3((p.sections - 1) * p.heads, walks),
+                         dim3(threads), row * (DK + DV), st, w);
     }
     const int64_t per_head = (int64_t)p.k.dim * p.v.dim;
     const int waves = (p.sections + DA_RUN - 2) / DA_RUN;
-    TMP_LAUNCH(decay_scan_kernel, dim3((unsigned)((per_head + 63) / 64 * p.heads)),
-               dim3((waves < DA_SCAN_WAVES ? waves : DA_SCAN_WAVES) * 64), st, p, per_head);
+    TMP_LAUNCH(decay_scan_kernel, dim3((unsigned)((per_head + 63) / 64 * p.heads), walks),
+               dim3((waves < DA_SCAN_WAVES ? waves : DA_SCAN_WAVES) * 64), st, w, per_head);
   }
   ProfScope ps("decay_walk_kernel", st);
-  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, true, EXACT>), dim3(p.sections * p.heads), dim3(threads),
-                     row * (2 * DK + DV), st, p);
+  hipLaunchKernelGGL(HIP_KERNEL_NAME(decay_walk_kernel<T, DK, DV, VEC, true, EXACT>), dim3(p.sections * p.heads, walks),
+                     dim3(threads), row * (2 * DK + DV), st, w);
 }
-template <typename T, int DK, int DV> static void decay_walk_form(const DecayParams &p, hipStream_t st) {
-  const bool vec = p.q.vec && p.k.vec && p.v.vec && p.out.vec;
+template <typename T, int DK, int DV> static void decay_walk_form(const DecayWalks &w, int walks, hipStream_t st) {
+  bool vec = true;
+  for (int i = 0; i < walks; ++i) vec = vec && w.p[i].q.vec && w.p[i].k.vec && w.p[i].v.vec && w.p[i].out.vec;
   constexpr bool SPLIT = sizeof(T) == 2;
-  if (SPLIT && p.state_out) {
-    if (vec) decay_walk<T, DK, DV, true, SPLIT>(p, st);
-    else decay_walk<T, DK, DV, false, SPLIT>(p, st);
+  if (SPLIT && w.p[0].state_out) {
+    if (vec) decay_walk<T, DK, DV, true, SPLIT>(w, walks, st);
+    else decay_walk<T, DK, DV, false, SPLIT>(w, walks, st);
   } else {
-    if (vec) decay_walk<T, DK, DV, true, false>(p, st);
-    else decay_walk<T, DK, DV, false, false>(p, st);
+    if (vec) decay_walk<T, DK, DV, true, false>(w, walks, st);
+    else decay_walk<T, DK, DV, false, false>(w, walks, st);
   }
 }
 // Both head sizes padded to 32, 64 or 128, and at most a factor of two apart.
-template <typename T> static void decay_walk_dims(const DecayParams &p, hipStream_t st) {
+template <typename T> static void decay_walk_dims(const DecayWalks &w, int walks, hipStream_t st) {
+  const DecayParams &p = w.p[0];
   int dk = padded_dim(p.k.dim), dv = padded_dim(p.v.dim);
   if (dk < dv / 2) dk = dv / 2;
   if (dv < dk / 2) dv = dk / 2;
   if (dk == 32) {
-    if (dv == 32) decay_walk_form<T, 32, 32>(p, st);
-    else decay_walk_form<T, 32, 64>(p, st);
+    if (dv == 32) decay_walk_form<T, 32, 32>(w, walks, st);
+    else decay_walk_form<T, 32, 64>(w, walks, st);
   } else if (dk == 64) {
-    if (dv == 32) decay_walk_form<T, 64, 32>(p, st);
-    else if (dv == 64) decay_walk_form<T, 64, 64>(p, st);
-    else decay_walk_form<T, 64, 128>(p, st);
+    if (dv == 32) decay_walk_form<T, 64, 32>(w, walks, st);
+    else if (dv == 64) decay_walk_form<T, 64, 64>(w, walks, st);
+    else decay_walk_form<T, 64, 128>(w, walks, st);
   } else {
-    if (dv == 64) decay_walk_form<T, 128, 64>(p, st);
-    else decay_walk_form<T, 128, 128>(p, st);
+    if (dv == 64) decay_walk_form<T, 128, 64>(w, walks, st);
+    else decay_walk_form<T, 128, 128>(w, walks, st);
   }
 }
-static void decay_run(const DecayParams &p, int type, hipStream_t st) {
-  if (type == TMP_F32) decay_walk_dims<float>(p, st);
-  else decay_walk_dims<__bf16>(p, st);
+// `walks` of w, all of the same padded head sizes and with a state returned by all or none.
+static void decay_run(const DecayWalks &w, int walks, int type, hipStream_t st) {
+  if (type == TMP_F32) decay_walk_dims<float>(w, walks, st);
+  else decay_walk_dims<__bf16>(w, walks, st);
 }
 
-static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d) {
+static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d, int walk) {
   DecayParams p;
   memset(&p, 0, sizeof(p));
   p.s.offsets = a->offsets; p.s.n_series = a->offsets ? a->n_series : 1; p.s.n = (int32_t)a->n;
   p.log_decay = a->log_decay;
-  p.carry = d.carry; p.link = d.link; p.section = d.section; p.sections = d.sections;
+  p.carry = d.carry + walk * d.per_walk; p.link = d.link + walk * (d.sections + 1); p.section = d.section; p.sections = d.sections;
   // Few rows in many series: one launch, whose blocks walk the rows of their first series that lie before them once
   // more, costs less than three (2000 rows of 100 series, 4 heads of 64: 20 us against 29 us); a single series would
   // make the last block walk all of them.
@@ -524,7 +537,7 @@ extern "C" size_t tmp_decay_attention_workspace_bytes(const tmp_decay_attention_
   if (!a || a->heads < 1 || a->dim_k < 1 || a->dim_v < 1) return 0;
   Workspace ws(nullptr, 0);
   DecayPlan d;
-  decay_plan(a, ws, &d);
+  decay_plan(a, a->dout.p || a->n <= 0 ? 3 : 1, ws, &d);  // (without rows there may be no pointers)
   return ws.off;
 }
 
@@ -533,11 +546,13 @@ extern "C" int tmp_decay_attention(const tmp_decay_attention_args *a, void *work
   TMP_TRY(decay_check(a, "tmp_decay_attention", false));
   Workspace ws(workspace, workspace_bytes);
   DecayPlan d;
-  decay_plan(a, ws, &d);
+  decay_plan(a, 1, ws, &d);
   TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_decay_attention: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   const int b = a->type == TMP_F32 ? 4 : 2;
-  DecayParams p = decay_params(a, d);
+  DecayWalks w = {};
+  DecayParams &p = w.p[0];
+  p = decay_params(a, d, 0);
   const char *what = "tmp_decay_attention";
   if (a->n > 0) {
     TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p.q);
@@ -546,7 +561,7 @@ extern "C" int tmp_decay_attention(const tmp_decay_attention_args *a, void *work
     TMP_ROWS(what, a->out, a->n, a->dim_v, b, &p.out);
   }
   p.state_in = a->state_in; p.state_out = a->state_out;
-  if (a->n > 0) decay_run(p, a->type, st);
+  if (a->n > 0) decay_run(w, 1, a->type, st);
   TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
@@ -557,7 +572,7 @@ extern "C" int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void 
   TMP_TRY(decay_check(a, "tmp_decay_attention_grad", true));
   Workspace ws(workspace, workspace_bytes);
   DecayPlan d;
-  decay_plan(a, ws, &d);
+  decay_plan(a, 3, ws, &d);
   TMP_REQUIRE(workspace && !ws.overflow(), TMP_EWORKSPACE, "tmp_decay_attention_grad: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   const int b = a->type == TMP_F32 ? 4 : 2;
@@ -572,22 +587,29 @@ extern "C" int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void 
     TMP_ROWS(what, a->dk, a->n, a->dim_k, b, &dk);
     TMP_ROWS(what, a->dv, a->n, a->dim_v, b, &dv);
   }
-  DecayParams p = decay_params(a, d);
-  if (a->n > 0) {
-    p.q = o; p.k = v; p.v = k; p.out = dq;
-    p.state_in = a->state_in; p.transposed = 1;
-    decay_run(p, a->type, st);
+  // The three walks do not depend on each other: those whose kernel is the same go in one launch
+  // (training of 24184 x 1 x 84/104: 224 us with three, 158 us so; of 50000 x 16 x 64: 605 us and 555 us).
+  DecayWalks w = {};
+  for (int i = 0; i < 3; ++i) w.p[i] = decay_params(a, d, i);
+  DecayParams &p0 = w.p[0], &p1 = w.p[1], &p2 = w.p[2];
+  p0.q = o; p0.k = v; p0.v = k; p0.out = dq;
+  p0.state_in = a->state_in; p0.transposed = 1;
+  p1.q = v; p1.k = o; p1.v = q; p1.out = dk; p1.transposed = 1;
+  p2.q = k; p2.k = q; p2.v = o; p2.out = dv;
+  for (int i = 1; i < 3; ++i) {
+    w.p[i].reverse = 1; w.p[i].state_in = a->dstate_out; w.p[i].in_by = 1.f / a->scale; w.p[i].out_by = a->scale;
   }
-  p.reverse = 1; p.state_in = a->dstate_out; p.in_by = 1.f / a->scale; p.out_by = a->scale;
+  p2.state_out = a->dstate_in;
   if (a->n > 0) {
-    p.q = v; p.k = o; p.v = q; p.out = dk;
-    decay_run(p, a->type, st);
-    p.q = k; p.k = q; p.v = o; p.out = dv;
-    p.transposed = 0; p.state_out = a->dstate_in;
-    decay_run(p, a->type, st);
+    const bool one = !p2.state_out && padded_dim(a->dim_k) == padded_dim(a->dim_v);
+    decay_run(w, one ? 3 : 2, a->type, st);
+    if (!one) {
+      DecayWalks last = {};
+      last.p[0] = p2;
+      decay_run(last, 1, a->type, st);
+    }
   }
-  p.state_out = a->dstate_in;
-  TMP_TRY(decay_empty(p, p.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
+  TMP_TRY(decay_empty(p2, p2.s.n_series, (int64_t)a->heads * a->dim_k * a->dim_v, st));
   TMP_CHECK_HIP(hipGetLastError());
   return TMP_OK;
 }
