@@ -751,7 +751,8 @@ int tmp_arrow_import(const struct ArrowArray *array, const struct ArrowSchema *s
  * offsets: one series of all rows.
  *
  * Row arrays: element d of head h of row r at p[r * row_stride + h * head_stride + d] (strides in
- * elements), of type TMP_BF16 or TMP_F32.  Sums, softmax statistics and states are 32-bit floats.
+ * elements), of type TMP_BF16 or TMP_F32; row_stride (the cache's too) is at least the head size and
+ * below 2^22, p a multiple of the type's size.  Outputs overlap neither an input nor each other.  Sums, softmax statistics and states are 32-bit floats.
  * A value that is not finite makes the results that depend on it not finite (NaN or infinite), and
  * no other ones.  Calls enqueue work and return; none of them waits for the device.
  */
@@ -759,6 +760,7 @@ int tmp_arrow_import(const struct ArrowArray *array, const struct ArrowSchema *s
 #define TMP_F32 1
 #define TMP_MAX_HEAD_DIM 128
 #define TMP_MAX_SINKS 32
+#define TMP_MAX_SLOT_ROWS 65536
 
 typedef struct {
   void *p;
@@ -774,7 +776,7 @@ typedef struct {
  *
  * _grad: dq, dk, dv from dout and, when dstate_out is given, the gradient of state_out; dstate_in
  * (NULL: not wanted) receives the gradient of state_in.  log_decay has no gradient.  out / state_out
- * are not read.  The workspace is the same for both.
+ * are not read.
  */
 typedef struct {
   int64_t n;
@@ -829,7 +831,8 @@ int tmp_window_attention_grad(const tmp_window_attention_args *a, void *workspac
  * rows seen so far.  Row t of a series lies at place t (t < sinks) or sinks + (t - sinks) % window.
  * Row b of the call is the next row of slot slots[b] (NULL: slot b): it is added first, then read with the
  * others, and the slot is changed in place.  A row whose slot is outside [0, n_slots) or is named by an
- * earlier row of the same call changes nothing and results in NaN.
+ * earlier row of the same call changes nothing and results in NaN.  With slots a call has at most
+ * TMP_MAX_SLOT_ROWS rows (series).
  *
  * tmp_window_cache_write fills slots from whole series (the rows that tmp_window_attention was called
  * on): slot slots[s] (NULL: s) afterwards holds series s and nothing else.  A series whose slot is out of

@@ -340,11 +340,13 @@ static bool cache_rows(const tmp_cache &c, int dim, int bytes, Rows *o) {
 }
 #define TMP_CACHE(what, ref, dim, bytes, to)                                                                   \
   TMP_REQUIRE(cache_rows(ref, dim, bytes, to), TMP_EUNSUPPORTED,                                               \
-              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements", what)
+              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements, its pointer aligned", what)
 
 static int step_check_common(int64_t n, int32_t n_slots, const int32_t *slots, int type, int heads, int dk, int dv,
                              const char *what) {
   TMP_REQUIRE(n >= 0 && n <= (1 << 24), TMP_EINVAL, "%s: row count must be in [0, 2^24]", what);
+  // (every row looks through the slots of those before it)
+  TMP_REQUIRE(!slots || n <= TMP_MAX_SLOT_ROWS, TMP_EUNSUPPORTED, "%s: at most %d rows with slots", what, TMP_MAX_SLOT_ROWS);
   TMP_REQUIRE(n_slots >= 0 && (slots || n <= n_slots), TMP_EINVAL, "%s: more rows than slots", what);
   TMP_REQUIRE(type == TMP_BF16 || type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
   TMP_REQUIRE(heads > 0 && heads <= 65536 && n * heads < (1ll << 31), TMP_EINVAL, "%s: bad number of heads", what);
@@ -397,6 +399,7 @@ extern "C" int tmp_decay_attention_step(const tmp_decay_attention_step_args *a, 
   const char *what = "tmp_decay_attention_step";
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_TRY(step_check_common(a->n, a->n_slots, a->slots, a->type, a->heads, a->dim_k, a->dim_v, what));
+  TMP_REQUIRE(a->scale > 0.f && a->scale < INFINITY, TMP_EINVAL, "%s: scale must be positive and finite", what);
   if (a->n == 0) return TMP_OK;
   TMP_REQUIRE(a->q.p && a->k.p && a->v.p && a->out.p && a->log_decay && a->state, TMP_EINVAL, "%s: null pointer", what);
   const int b = a->type == TMP_F32 ? 4 : 2;

@@ -451,11 +451,11 @@ inline bool rows_of(const tmp_rows &r, int64_t n, int dim, int bytes, Rows *o) {
   const int64_t per = 16 / bytes;
   o->p = r.p; o->row = n > 1 ? r.row_stride : (dim + 7) / 8 * 8; o->head = r.head_stride; o->dim = dim;
   o->vec = ((uintptr_t)r.p & 15) == 0 && o->row % per == 0 && r.head_stride % per == 0 && dim % 8 == 0;
-  return o->row >= dim && o->row < (1 << 22);
+  return o->row >= dim && o->row < (1 << 22) && (uintptr_t)r.p % bytes == 0;
 }
 #define TMP_ROWS(what, ref, n, dim, bytes, to)                                                                 \
   TMP_REQUIRE(rows_of(ref, n, dim, bytes, to), TMP_EUNSUPPORTED,                                               \
-              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements", what)
+              "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements, its pointer aligned", what)
 
 // fn<T, D, VEC>(...) for a type, a padded head size and an access width.
 #define TMP_BY_DIM(fn, T, d, VEC, ...)              \

@@ -140,6 +140,32 @@ def test_argument_errors_need_no_gpu():
     assert h.tmp_window_cache_write(C.byref(a), None) == -1 and b"series" in h.tmp_last_error()
 
 
+def test_what_a_step_cannot_take():
+    """Rows that would look through too many slots, arrays that do not lie at multiples of their type's size, scales."""
+    from tempo_amd import _lib
+    h = _lib.lib()
+    rows, cache = _lib.RowsRef(4096, 64, 16), _lib.CacheRef(4096, 640, 64, 16)
+    many = 65537
+    a = dict(n=many, n_slots=many, slots=4096, type=0, heads=1, dim_k=16, dim_v=16, scale=1.0, log_decay=4096, q=rows, k=rows,
+             v=rows, out=rows, state=4096)
+    for change, rc, text in [({}, -4, b"65536"), (dict(n=2, scale=0.0), -1, b"scale"), (dict(n=2, scale=math.nan), -1, b"scale"),
+                             (dict(n=2, k=_lib.RowsRef(4097, 64, 16)), -4, b"aligned"),
+                             (dict(n=2, type=1, v=_lib.RowsRef(4098, 64, 16)), -4, b"aligned")]:
+        assert h.tmp_decay_attention_step(C.byref(_struct(_lib.DecayAttentionStepArgs, **{**a, **change})), None) == rc, change
+        assert text in h.tmp_last_error(), (change, h.tmp_last_error())
+    a = dict(n=many, n_slots=many, slots=4096, type=0, heads=1, kv_heads=1, dim_k=16, dim_v=16, window=8, sinks=1, scale=1.0,
+             q=rows, k=rows, v=rows, out=rows, k_cache=cache, v_cache=cache, length=4096)
+    assert h.tmp_window_attention_step(C.byref(_struct(_lib.WindowAttentionStepArgs, **a)), None, 0, None) == -4
+    assert b"65536" in h.tmp_last_error()
+    a = dict(n=4, n_series=many, offsets=4096, n_slots=many, slots=4096, type=0, kv_heads=1, dim_k=16, dim_v=16, window=8, k=rows,
+             v=rows, k_cache=cache, v_cache=cache, length=4096)
+    assert h.tmp_window_cache_write(C.byref(_struct(_lib.WindowCacheWriteArgs, **a)), None) == -4
+    assert b"65536" in h.tmp_last_error()
+    a.update(n_series=2, v_cache=_lib.CacheRef(4097, 640, 64, 16))
+    assert h.tmp_window_cache_write(C.byref(_struct(_lib.WindowCacheWriteArgs, **a)), None) == -4
+    assert b"aligned" in h.tmp_last_error()
+
+
 def test_host_tensors_are_refused():
     from tempo_amd import ops
     t = torch.zeros(4, 2, 8)
