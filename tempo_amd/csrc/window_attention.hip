@@ -221,6 +221,10 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
   }
 }
 
+// Bound by the matrix cores and the vector unit together: an element of a part costs 4 D operations and some ten vector
+// instructions (scale, maximum, exponential, sum, rounding), which take as long as the products at D = 64 and half as
+// long at 128.  131072 x 16 x 128, window 600: 1.10 ms, 577 TFLOP/s of visible pairs; 32768 x 16 x 64, window 1000:
+// 216 us, 537 TFLOP/s (library products reach 1134).  Waves a SIMD: as many as fit the registers without spilling.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2) void window_forward_kernel(WindowParams p, int tiles) {
   // float: matrix instructions are a sixteenth as fast, and parts that a wave does not see are left out one by one
@@ -372,7 +376,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T
     p.lse[(int64_t)r.i * p.heads + head] = in ? (m + log2_hw(l)) * kLn2 : -INFINITY;
 }
 
-// dq, and do.o for the kernel that follows.
+// dq, and do.o for the kernel that follows.  Scores are computed again: 6 D operations for each element and no running
+// maximum.  32768 x 16 x 64, window 1000: 250 us, 697 TFLOP/s.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_dq_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.heads);
@@ -471,6 +476,7 @@ __device__ inline int last_query(const WindowParams &p, int j0) {
 // dk and dv: a block owns key rows and streams the query rows that see them, head after head of the
 // group that shares them.  SINK: the rows that stay visible, against the query rows of one section
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
+// 32768 x 16 x 64 sharing 4, window 1000: 354 us, 656 TFLOP/s (8 D operations an element); its four sinks 41 us.
 template <typename T, int D, bool VEC, bool SINK>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void window_dkdv_kernel(WindowParams p, int tiles) {
   // Float of 128: the own rows and both sums take 256 of the 512 registers.  Tiles of 32 rows, whose places in LDS are
@@ -647,7 +653,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 256 ? 1 : 2) void wind
 }
 
 // Adds up the parts of all sections that a series reaches into, in the place of the first of them.  A
-// block takes one (section, key/value head) and has work only where the section is such a first one.
+// block takes one (section, key/value head) and has work only where the section is such a first one (13 us there:
+// latency, eight sums a thread at a time).
 __global__ __launch_bounds__(256) void sink_sum_kernel(WindowParams p) {
   const int sec = blockIdx.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
   const int sec0 = sec * WA_SECTION;
