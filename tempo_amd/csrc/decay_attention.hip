@@ -92,7 +92,7 @@ template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], flo
 
 // X <- X + K^T diag(w) V for sixteen rows.  The weighted values do not fit bfloat16; they enter as the sum
 // of two such numbers (2^-18 of a term), three where the state itself is returned (2^-27).
-template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int k0, const float *w, bf16x8 v) {
+template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int k0, const float *w, bf16x8 v, int) {
   bf16x8 hi, lo;
   f32x8 x;
 #pragma unroll
@@ -115,17 +115,17 @@ template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 3
     if (EXACT) st[t] = mma(kf, rest, st[t]);
   }
 }
-template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const float *kt, int k0, const float *w, f32x8 v) {
+template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const float *kt, int k0, const float *w, f32x8 v, int l) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] *= w[e];
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, k0, 32 * t), v, st[t]);
+  for (int t = 0; t < D / 32; ++t) st[t] = mma(col_frag<D>(kt, k0, 32 * t, l), v, st[t]);
 }
 
-// Waves a SIMD: two where state, tiles on their way and decays fit 256 registers without spilling.
-constexpr int da_waves(int bytes, int dk, int dv, bool out) {
-  return (dk == 128 && bytes == 4) || dv < dk ? 1 : 2;
-}
+// Waves a SIMD: two where state, tiles on their way and decays fit 256 registers with next to no spilling.  Float of 128
+// fits because its places in LDS are worked out anew for each part (11071 x 15 x 104/80 training: 959 us with one wave,
+// 882 us with two).
+constexpr int da_waves(int dk, int dv) { return dv < dk ? 1 : 2; }
 
 // OUT: walks a section and writes its rows.  Otherwise: walks the rows of the section that belong to the
 // series which goes on behind it, and leaves the state that they make in carry[section + 1].
@@ -136,8 +136,9 @@ constexpr int da_waves(int bytes, int dk, int dv, bool out) {
 // 131072 x 16 x 128 bf16 514 us, 4.2 TB/s (states alone 224 us, 4.8 TB/s); 50000 x 16 x 64 bf16, the backward pass's
 // three 312 us, 3.9 TB/s; float by its matrix instructions (30011 x 8 x 40/72: 159 us).
 template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
-__global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void decay_walk_kernel(DecayWalks w) {
+__global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(DecayWalks w) {
   const DecayParams &p = w.p[blockIdx.y];
+  constexpr bool FRESH = DK * sizeof(T) >= 512;
   constexpr int NT = DK / 32, THREADS = DV * 2, SUB = 32, DA_PIECE = da_piece(sizeof(T), DK);
   const int sec = blockIdx.x / p.heads, head = blockIdx.x % p.heads;
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
@@ -265,6 +266,9 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
     }
 #pragma unroll 1
     for (int r0 = 0; r0 < len; r0 += SUB) {
+      int l = lane;
+      if (FRESH) asm volatile("" : "+v"(l));
+      const int l31 = l & 31, h8 = (l >> 5) * 8;
       const int rows = len - r0 < SUB ? len - r0 : SUB;
       if (OUT && pos >= sec0) {
         f32x16 acc = zero16(), s = zero16();
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
           s[x] = 16 * (x >> 3) + h8 + (x & 7) <= l31 ? s[x] * (TABLE ? within[x >> 2][lane][x & 3] : wd[x]) : 0.f;
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc = mma(col_frag<DV>(vt, r0 + 16 * b, strip), operand<T>(s, b), acc);
+        for (int b = 0; b < 2; ++b) acc = mma(col_frag<DV>(vt, r0 + 16 * b, strip, l), operand<T>(s, b), acc);
         if (__builtin_expect(dirty, 0)) {  // they reach the rows at and behind their own, as NaN
           const int first = r0 ? bad[1] : bad[0];
 #pragma unroll
@@ -310,7 +314,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
           float w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = TABLE ? behind[lane >> 5][2 * b + (e >> 2)][e & 3] : w_all[8 * b + e];
-          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip));
+          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip, l), l);
         }
       } else {
 #pragma unroll 1
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(sizeof(T), DK, DV, OUT)) void deca
             const int left = rows - 1 - (16 * b + h8 + e);
             w[e] = left >= 0 ? power(ld, left + post) : 0.f;
           }
-          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip));
+          state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip, l), l);
         }
       }
       if (__builtin_expect(dirty, 0)) {
@@ -411,13 +415,10 @@ __global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t
 
 // Sections of whole pieces, as few as give the 1024 SIMDs the two waves each that they hold (a block has one for 32 of
 // dv): every one more adds a state to be written, strung together and read.  131072 x 16 x 128 bf16: 512 blocks 913 us,
-// 1024 955 us, 2048 1017 us; 50000 x 16 x 64: a walk takes 113 us with 1024 or 2048 blocks, 120 us with 512.  Float
-// with both sizes above 64 has one wave a SIMD: 14350 x 3 x 116/71 training 603 us with 512 blocks, 465 us with 256
-// (and 30011 x 8 x 40/72, two waves: 237 us with 512, 283 us with 256).
-static int decay_section(int64_t n, int heads, int dim_k, int dim_v, int bytes) {
-  const int dk = padded_dim(dim_k), dv = padded_dim(dim_v);
-  const int least = dk < dv ? dk : dv, most = dk < dv ? dv : dk;  // (either is the values' in some walk)
-  const int blocks = (bytes == 4 && least == 128 ? 1024 : 2048) / (most / 32);
+// 1024 955 us, 2048 1017 us; 50000 x 16 x 64: a walk takes 113 us with 1024 or 2048 blocks, 120 us with 512.
+static int decay_section(int64_t n, int heads, int dim) {
+  const int dv = padded_dim(dim);  // the larger of the two sizes: either is the values' in some walk
+  const int blocks = 2048 / (dv / 32);
   int64_t s = (n * heads + blocks - 1) / blocks;
   if (s > n) s = n;
   s = (s + 63) / 64 * 64;
@@ -433,7 +434,7 @@ struct DecayPlan {
 };
 static void decay_plan(const tmp_decay_attention_args *a, int walks, Workspace &ws, DecayPlan *d) {
   const int64_t n = a->n > 0 ? a->n : 1;
-  d->section = decay_section(n, a->heads, a->dim_k, a->dim_v, a->type == TMP_F32 ? 4 : 2);
+  d->section = decay_section(n, a->heads, a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
   d->sections = (int)((n + d->section - 1) / d->section);
   d->per_walk = (size_t)d->sections * a->heads * a->dim_k * a->dim_v;
   d->carry = ws.take<float>(d->per_walk * walks);

@@ -257,6 +257,7 @@ template <int D> __device__ inline bf16x8 col_frag(const __bf16 *t, int k0, int 
   for (int e = 0; e < 4; ++e) { f[e] = lo[e]; f[e + 4] = hi[e]; }
   return __builtin_bit_cast(bf16x8, f);
 }
+template <int D> __device__ inline bf16x8 col_frag(const __bf16 *t, int k0, int d0, int) { return col_frag<D>(t, k0, d0); }
 template <int D> __device__ inline f32x8 col_frag(const float *t, int k0, int d0, int l = lane_id()) {
   const int d = d0 + pi_of(l & 31), row = k0 + ((l >> 5) << 3);
   f32x8 f;
