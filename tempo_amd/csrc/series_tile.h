@@ -189,7 +189,8 @@ template <typename T> __device__ inline Frag<T> buffer_load8(Run u, uint32_t at,
   return vec ? f : settled(f, fifth, (u.lead + at) & 3, dim - d);
 }
 
-// Whole pieces at a word's start in one or two stores; the others element by element.
+// Whole pieces in one or two stores, bfloat16 at an odd place in three (its second to seventh elements are words); what
+// ends the row element by element.
 template <typename T> __device__ inline void buffer_store8(Run u, uint32_t at, int d, int dim, bool vec, Frag<T> f) {
   const uint32_t o = (vec ? at : u.lead + at) + d * (uint32_t)sizeof(T);
   const bool whole = vec ? d < dim : d + 8 <= dim && (o & 3) == 0;
@@ -198,6 +199,18 @@ template <typename T> __device__ inline void buffer_store8(Run u, uint32_t at, i
 #pragma unroll
   for (int c = 0; c < (int)sizeof(T) / 2; ++c) __builtin_amdgcn_raw_buffer_store_b128(w[c], u.b, whole ? o + 16 * c : kOutside, 0, 0);
   if (vec || whole || d >= dim) return;
+  if constexpr (sizeof(T) == 2) {
+    if (d + 8 <= dim) {
+      typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+      u32x3 x;
+#pragma unroll
+      for (int c = 0; c < 3; ++c) x[c] = __builtin_amdgcn_alignbyte(w[0][c + 1], w[0][c], 2);
+      __builtin_amdgcn_raw_buffer_store_b16((short)w[0][0], u.b, o, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b96(x, u.b, o + 2, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b16((short)(w[0][3] >> 16), u.b, o + 14, 0, 0);
+      return;
+    }
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const T x = f[e];
