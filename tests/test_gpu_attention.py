@@ -592,3 +592,75 @@ def test_refused_on_the_device():
         ops.window_attention_step(q[:3], k[:3], v[:3], cache[:1].expand(3, 8, 2, 16), cache, length)
     with pytest.raises(ValueError, match="gradient"):
         ops.decay_attention_step(q.requires_grad_(), q, q, ld, torch.zeros(10, 4, 16, 16, device="cuda"))
+
+
+def _among_nan(t, lead, gap):
+    """t [rows, heads, dim] on the device as a view whose every neighbour in memory is NaN: `lead` elements before, `gap`
+    behind each head, gap + 3 more behind each row."""
+    n, h, d = t.shape
+    row = h * (d + gap) + gap + 3
+    flat = torch.full((lead + n * row + 16,), math.nan, dtype=t.dtype, device="cuda")
+    view = flat.as_strided((n, h, d), (row, d + gap, 1), lead)
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv,lead,gap", [(5, 9, 1, 1), (40, 33, 3, 0), (64, 64, 1, 0), (127, 121, 5, 2), (128, 128, 7, 3),
+                                            (16, 24, 2, 6)])
+def test_neighbours_in_memory_do_not_show(dk, dv, lead, gap, dtype):
+    """Rows at every odd place, NaN all around them: whole forms, their gradients, and steps over such rows and caches."""
+    from tempo_amd import ops
+    off = [0, 1, 131, 131, 333]
+    n, h, window, sinks = off[-1], 2, 40, 3
+    o = torch.tensor(off, device="cuda")
+    q, k, v, do = _inputs(dk * 3 + dv, n, h, h, dk, dv, dtype)
+    scale = dk ** -0.5
+    qd, kd, vd, dod = [_among_nan(x.cuda(), lead, gap) for x in (q, k, v, do)]
+    want = ref.window_reference(q, k, v, do, off, window, sinks, scale)
+    out, lse = ops.window_attention(qd, kd, vd, window, sinks=sinks, offsets=o, return_lse=True)
+    ref.check("out", out, *want["out"])
+    for name, x in zip(("dq", "dk", "dv"), ops.window_attention_grad(dod, qd, kd, vd, _among_nan(out, lead, gap), lse, window,
+                                                                      sinks=sinks, offsets=o)):
+        ref.check(name, x, *want[name])
+    ld = torch.tensor([-0.2, -0.003])
+    decay = ref.decay_reference(q, k, v, ld, off, scale, dout=do)
+    ref.check("decay out", ops.decay_attention(qd, kd, vd, ld.cuda(), offsets=o), *decay["out"])
+    for name, x in zip(("dq", "dk", "dv"), ops.decay_attention_grad(dod, qd, kd, vd, ld.cuda(), offsets=o)):
+        ref.check("decay " + name, x, *decay[name])
+    # caches whose every row lies among NaN, filled from all rows but each series' last, which the step adds
+    rows = window + sinks
+    caches = []
+    for d in (dk, dv):
+        step = h * (d + gap) + gap + 3
+        flat = torch.full((lead + 4 * rows * step + 16,), math.nan, dtype=dtype, device="cuda")
+        caches.append(flat.as_strided((4, rows, h, d), (rows * step, step, d + gap, 1), lead))
+    length = torch.zeros(4, dtype=torch.int64, device="cuda")
+    old = torch.cat([torch.arange(off[i], max(off[i], off[i + 1] - 1)) for i in range(4)])
+    o_old = torch.tensor(_offsets([max(0, off[i + 1] - off[i] - 1) for i in range(4)]), device="cuda")
+    ops.window_cache_write(kd[old.cuda()], vd[old.cuda()], *caches, length, sinks=sinks, offsets=o_old)
+    has = [0, 1, 3]
+    last = torch.tensor([off[i + 1] - 1 for i in has])
+    got = ops.window_attention_step(*[_among_nan(x[last.cuda()], lead, gap) for x in (qd, kd, vd)], *caches, length, sinks=sinks,
+                                    slots=torch.tensor(has, dtype=torch.int32, device="cuda"))
+    ref.check("step", got, want["out"][0][last], want["out"][1][last])
+    for c, d in zip(caches, (dk, dv)):  # nothing between the rows was written
+        flat = torch.as_strided(c, (lead + 4 * c.stride(0) + 16,), (1,), 0)
+        kept = torch.ones_like(flat, dtype=torch.bool)
+        torch.as_strided(kept, c.shape, c.stride(), lead).fill_(False)
+        assert bool(flat[kept].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,dk,dv", [(3, 64, 48), (1, 128, 70), (5, 17, 32), (2, 100, 40)])
+def test_decay_gradients_without_states(heads, dk, dv, dtype):
+    """Long and short series, no state given or wanted: the walks that share a launch, over several sections."""
+    from tempo_amd import ops
+    off = _offsets([900, 1, 0, 64, 2500, 31, 700])
+    n = off[-1]
+    q, k, v, do = _inputs(heads + dk, n, heads, heads, dk, dv, dtype)
+    ld = torch.linspace(-0.5, -0.001, heads)
+    want = ref.decay_reference(q, k, v, ld, off, dk ** -0.5, dout=do)
+    d, o = _dev(q, k, v, do), torch.tensor(off, device="cuda")
+    for name, x in zip(("dq", "dk", "dv"), ops.decay_attention_grad(d[3], *d[:3], ld.cuda(), offsets=o)):
+        ref.check(name, x, *want[name])
