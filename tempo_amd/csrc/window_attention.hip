@@ -226,9 +226,12 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
 // long at 128.  131072 x 16 x 128, window 600: 1.10 ms, 577 TFLOP/s of visible pairs; 32768 x 16 x 64, window 1000:
 // 216 us, 537 TFLOP/s (library products reach 1134).  Waves a SIMD: as many as fit the registers without spilling.
 template <typename T, int D, bool VEC>
-__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T) == 128 ? 3 : 2) void window_forward_kernel(WindowParams p, int tiles) {
+__global__ __launch_bounds__(WA_THREADS, D * sizeof(T) == 128 ? 3 : 2) void window_forward_kernel(WindowParams p, int tiles) {
   // float: matrix instructions are a sixteenth as fast, and parts that a wave does not see are left out one by one
   constexpr int PARTS = sizeof(T) == 4 ? 1 : 2;
+  // float of 128: places in LDS worked out anew for each part leave registers enough for a second wave a SIMD
+  // (89835 x 9 sharing 3, window 504: 2.18 ms with one, 1.92 ms with two)
+  constexpr bool TIGHT = sizeof(T) == 4 && D == 128;
   const int item = item_of_block(tiles * p.heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
@@ -328,11 +331,23 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : D * sizeof(T
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (!r.any(p, j0 + u * 32, 32)) continue;
-        scores(u);
-        mask(u);
-        maximum(s[u], false);
-        weights(u);
-        add_rows<T, D>(acc, vt, u * 32, s[u]);
+        if constexpr (TIGHT) {
+          int l = lane_id();
+          asm volatile("" : "+v"(l));
+          s[u] = zero16();
+#pragma unroll
+          for (int b = 0; b < D / 16; ++b) s[u] = mma(row_frag<D>(kt, u * 32 + pi_of(l & 31), 16 * b + (l >> 5) * 8), qf[b], s[u]);
+          mask(u);
+          maximum(s[u], false);
+          weights(u);
+          add_rows_at<D>(acc, vt, u * 32, s[u], l);
+        } else {
+          scores(u);
+          mask(u);
+          maximum(s[u], false);
+          weights(u);
+          add_rows<T, D>(acc, vt, u * 32, s[u]);
+        }
       }
     } else if (D == 128) {
       constexpr int N = D / 16, VALU = 64 / N;
