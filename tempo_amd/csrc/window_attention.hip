@@ -491,18 +491,18 @@ __device__ inline int last_query(const WindowParams &p, int j0) {
 // Waves a SIMD of the kernel below, and whether its places in LDS are worked out anew for each part, which frees the
 // registers that hold them (float's many matrix instructions leave the time).  Float of 64 gets its second wave so
 // (5170 x 28 x 33, window 88: 305 us with one wave, 327 us with one and new places, 311 us with two and old ones, 248 us
-// so); float of 128 spills less (7950 x 28 x 128, window 94: 1103 us otherwise, 650 us with tiles of 32 rows besides).
-constexpr bool wa_tight(int bytes, int d, bool sink) { return bytes == 4 && d >= 64 && !sink; }
-constexpr int wa_waves(int bytes, int d, bool sink) { return d * bytes < 256 || (d * bytes == 256 && wa_tight(bytes, d, sink)) ? 2 : 1; }
+// so); float of 128 spills less (7950 x 28 x 128, window 94: 1103 us otherwise, 635 us with tiles of 32 rows besides; its sinks 309 and 256 us).
+constexpr bool wa_tight(int bytes, int d) { return bytes == 4 && d >= 64; }
+constexpr int wa_waves(int bytes, int d) { return d * bytes < 256 || (d * bytes == 256 && wa_tight(bytes, d)) ? 2 : 1; }
 
 // dk and dv: a block owns key rows and streams the query rows that see them, head after head of the
 // group that shares them.  SINK: the rows that stay visible, against the query rows of one section
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
 // 32768 x 16 x 64 sharing 4, window 1000: 354 us, 656 TFLOP/s (8 D operations an element); its four sinks 41 us.
 template <typename T, int D, bool VEC, bool SINK>
-__global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D, SINK)) void window_dkdv_kernel(WindowParams p, int tiles) {
-  constexpr bool TIGHT = wa_tight(sizeof(T), D, SINK);
-  constexpr int TILE = TIGHT && D == 128 ? 32 : WA_TILE;
+__global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkdv_kernel(WindowParams p, int tiles) {
+  constexpr bool TIGHT = wa_tight(sizeof(T), D);
+  constexpr int TILE = TIGHT && D == 128 && !SINK ? 32 : WA_TILE;  // (a section's two waves take a part each of 64)
   const int item = item_of_block(tiles * p.kv_heads);
   if (item < 0) return;
   const int group = p.heads / p.kv_heads;
