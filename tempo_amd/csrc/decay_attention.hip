@@ -134,7 +134,7 @@ constexpr int da_waves(int dk, int dv) { return dv < dk ? 1 : 2; }
 // values' tiles (da_piece rows) are shared, the next ones on their way meanwhile.  Rows are worked on in parts of
 // SUB, whose decays are the same for every part but a series' last one.  Memory bounds it once there are rows enough:
 // 131072 x 16 x 128 bf16 514 us, 4.2 TB/s (states alone 224 us, 4.8 TB/s); 50000 x 16 x 64 bf16, the backward pass's
-// three 312 us, 3.9 TB/s; float by its matrix instructions (30011 x 8 x 40/72: 159 us).
+// three 312 us, 3.9 TB/s; float by its matrix instructions (30011 x 8 x 40/72: 150 us).
 template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
 __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(DecayWalks w) {
   const DecayParams &p = w.p[blockIdx.y];
@@ -436,7 +436,7 @@ static void decay_plan(const tmp_decay_attention_args *a, int walks, Workspace &
   const int64_t n = a->n > 0 ? a->n : 1;
   d->section = decay_section(n, a->heads, a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
   d->sections = (int)((n + d->section - 1) / d->section);
-  d->per_walk = (size_t)d->sections * a->heads * a->dim_k * a->dim_v;
+  d->per_walk = d->sections > 1 ? (size_t)d->sections * a->heads * a->dim_k * a->dim_v : 0;  // (nothing is carried)
   d->carry = ws.take<float>(d->per_walk * walks);
   d->link = ws.take<int32_t>((size_t)(d->sections + 1) * walks);
 }

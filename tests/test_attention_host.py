@@ -175,3 +175,12 @@ def test_host_tensors_are_refused():
         ops.decay_attention(t, t, t, torch.zeros(2))
     with pytest.raises(TypeError, match="no CPU path"):
         ops.decay_attention_step(t, t, t, torch.zeros(2), torch.zeros(4, 2, 8, 8))
+
+
+def test_one_section_carries_nothing():
+    from tempo_amd import _lib
+    h = _lib.lib()
+    a = _struct(_lib.DecayAttentionArgs, n=64, heads=4096, dim_k=128, dim_v=128, dout=_lib.RowsRef(4096, 64, 16))
+    assert h.tmp_decay_attention_workspace_bytes(C.byref(a)) < 1 << 12
+    a.n, a.heads = 100_000, 2
+    assert h.tmp_decay_attention_workspace_bytes(C.byref(a)) >= 3 * 2 * 2 * 128 * 128 * 4
