@@ -233,7 +233,7 @@ def _no_grad(*tensors):
 def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One new row for each of some series: q, k [b, heads, dk], v [b, heads, dv]; state float32 [n_slots, heads,
     dk, dv], changed in place; slots int32 [b] (None: row i is slot i).  A row whose slot is out of range or named
-    by an earlier row changes nothing and results in NaN.  Returns out [b, heads, dv]."""
+    by an earlier row changes nothing and results in NaN; with slots b is at most 65536.  Returns out [b, heads, dv]."""
     q = _rows_check(q, "q")
     n, heads, dk = q.shape
     k = _rows_check(k, "k", q, n, heads, dk)
@@ -379,7 +379,8 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
     """One new row for each of some series: adds k, v [b, kv_heads, dim] to the caches (in place, length counts
     it) and attends with q [b, heads, dk] over the slot's last `window` rows, the new one included, and its first
     `sinks`.  The caches' number of rows is window + sinks.  slots int32 [b] (None: row i is slot i); a row whose slot is
-    out of range or named by an earlier row changes nothing and results in NaN.  Returns out [b, heads, dv]."""
+    out of range or named by an earlier row changes nothing and results in NaN; with slots b is at most 65536.  Returns
+    out [b, heads, dv]."""
     q = _rows_check(q, "q")
     n, heads, dk = q.shape
     k = _rows_check(k, "k", q, n, None, dk)

@@ -664,3 +664,40 @@ def test_decay_gradients_without_states(heads, dk, dv, dtype):
     d, o = _dev(q, k, v, do), torch.tensor(off, device="cuda")
     for name, x in zip(("dq", "dk", "dv"), ops.decay_attention_grad(d[3], *d[:3], ld.cuda(), offsets=o)):
         ref.check(name, x, *want[name])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf], ids=["nan", "inf"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (24, 70)])
+def test_values_that_are_not_finite_and_states_between_sections(dk, dv, dtype, bad):
+    """Series over many sections, whose states are strung together: a bad element shows in its series from its row on
+    (in gradients of keys and values up to it) and nowhere else."""
+    from tempo_amd import ops
+    off = _offsets([300, 1100, 40, 700])
+    n, h, head = off[-1], 2, 1
+    o = torch.tensor(off, device="cuda")
+    clean = _inputs(dk + dv, n, h, h, dk, dv, dtype)
+    ld = torch.tensor([-0.1, -0.02]).cuda()
+    sid, _ = ref.series_of(n, off)
+    at = torch.arange(n)
+
+    def run(ts):
+        q, k, v, do = _dev(*ts)
+        res = [ops.decay_attention(q, k, v, ld, offsets=o), *ops.decay_attention_grad(do, q, k, v, ld, offsets=o)]
+        return [x.float().cpu() for x in res]
+
+    base = run(clean)
+    for which, row in ((0, 700), (1, 310), (1, 1399), (2, 655), (2, 1500), (3, 900)):
+        ts = [x.clone() for x in clean]
+        ts[which][row, head, 5] = bad
+        got = run(ts)
+        behind, before = (sid == sid[row]) & (at >= row), (sid == sid[row]) & (at <= row)
+        # out, dq, dk, dv: which rows each may differ in, and which of them are certainly not finite
+        reach = {0: (at == row, at == at.new_tensor(-1), before, before), 1: (behind, behind, at == row, before),
+                 2: (behind, behind, before, at == row), 3: (at == at.new_tensor(-1), at == row, before, before)}[which]
+        for name, x, y, rows in zip(("out", "dq", "dk", "dv"), got, base, reach):
+            where = torch.zeros(n, h, dtype=torch.bool)
+            where[:, head] = rows
+            assert torch.equal(x[~where], y[~where]), (which, row, name)
+        if which < 3:
+            assert not bool(got[0][reach[0]][:, head].isfinite().all(-1).any()), (which, row)
