@@ -21,8 +21,10 @@ constexpr int WA_TILE = 64;    // rows of a streamed tile
 constexpr int WA_THREADS = 256;
 constexpr int WA_SECTION = WA_OWN;  // query rows whose share of the sinks' gradients one block adds up
 
-// Up to this window dS enters its products as two bfloat16 numbers: with few rows the error of do.o (of the rounded out)
-// is large beside dS, and a second rounding would show (error against 64 bits at window 11: 2.6e-3 with one number).
+// bfloat16: dS enters dq as the sum of two numbers, since its own rounding would come on top of that of do.o (of the
+// rounded out): error against 64 bits at window 1000, head size 64 1.82e-3, 2.48e-3 with one number (rounding dq itself
+// is 1.65e-3); 32768 x 16 x 64: 294 us, 250 us with one.  For dk, whose do.o are many rows', it does so up to this
+// window (11: 2.00e-3 and 2.60e-3, dk and dv there 6 % slower); beyond, one number costs less than it saves.
 constexpr int WA_FINE = 64;
 
 struct WindowParams {
@@ -392,7 +394,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) == 128 ? 3 : 2) void wind
 }
 
 // dq, and do.o for the kernel that follows.  Scores are computed again: 6 D operations for each element and no running
-// maximum.  32768 x 16 x 64, window 1000: 250 us, 697 TFLOP/s.
+// maximum, and 2 D more for the rest of dS.  32768 x 16 x 64, window 1000: 294 us, 790 TFLOP/s with those.
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_dq_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.heads);
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
         else mask_part<false>(s, seen, u * 32 + h8, 0.f);
       }
       add_rows<T, D>(acc, kt, u * 32, s);
-      if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(acc, kt, u * 32, left_over<T>(s));
+      if (sizeof(T) == 2) add_rows<T, D>(acc, kt, u * 32, left_over<T>(s));
     }
   }
   store_own<T, D, VEC>(acc, p.scale, p.dq, rows_buffer<T>(p.dq, head, t0, own), r.i - t0);
