@@ -12,6 +12,7 @@
 // sum of the softmax are lane-local but for one exchange, and scores turn into operands in place.
 #include <string.h>
 
+#include "row_limits.h"
 #include "series_tile.h"
 
 namespace tmp {
@@ -485,10 +486,7 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void wind
 
 // Last query row + 1 whose pairs with the key rows of tile [j0, j0 + WA_OWN) the main dk/dv kernel adds: the window's.
 // Pairs of rows that stay visible with later rows are the sink kernel's.
-__device__ inline int last_query(const WindowParams &p, int j0) {
-  const int64_t hi = (int64_t)j0 + WA_OWN + p.window - 1;
-  return hi < p.s.n ? (int)hi : p.s.n;
-}
+__device__ inline int last_query(const WindowParams &p, int j0) { return window_end(j0, WA_OWN, p.window, p.s.n); }
 
 // Waves a SIMD of the kernel below, and whether its places in LDS are worked out anew for each part, which frees the
 // registers that hold them (float's many matrix instructions leave the time).  Float of 64 gets its second wave so
@@ -586,7 +584,7 @@ __global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkd
     __syncthreads();
     // query rows [first, last] of a tile see key row j: those of its window, all behind it if it stays visible
     const int last = min_of(end, i1) - 1 - r0;
-    const Seen seen = {max_of(j, from) - r0, min_of(j < start + p.sinks ? last : j + p.window - 1 - r0, last), 0, -1};
+    const Seen seen = {max_of(j, from) - r0, min_of(j < start + p.sinks ? last : window_reach(j, r0, p.window), last), 0, -1};
     if (__builtin_expect(flag[t & 1], 0)) {
       if (!SINK || wave == 0) {  // (two waves share a section's rows: the first speaks for both)
         add_not_finite<T, D, TILE>(dv, dt, seen);
@@ -607,7 +605,7 @@ __global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkd
         if (wave != (ru - i0) / 32 % 2 || ru + 32 <= wfirst) continue;  // two waves share the section's rows
       } else {
         if (ru + 31 < wmin_j || ru >= wend) continue;
-        if (!wsink && ru > wmax_j + p.window - 1) continue;
+        if (!wsink && beyond_window(ru, wmax_j, p.window)) continue;
       }
       int l = lane;
       if (TIGHT) asm volatile("" : "+v"(l));
@@ -624,7 +622,7 @@ __global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkd
         s[x] = exp2_hw(__builtin_fmaf(s[x], c, -lse_t[row]));
         dp[x] = s[x] * (dp[x] - delta_t[row]);
       }
-      if (!(wall && ru >= wmax_j && ru >= wfrom && ru + 31 < wlast && ru + 31 < wmin_j + p.window)) {
+      if (!(wall && ru >= wmax_j && ru >= wfrom && ru + 31 < wlast && !beyond_window(ru + 31, wmin_j, p.window))) {
         asm volatile("");
         mask_part<false>(s, seen, u * 32 + h8, 0.f);
         mask_part<false>(dp, seen, u * 32 + h8, 0.f);
