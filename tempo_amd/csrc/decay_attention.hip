@@ -19,6 +19,7 @@
 // series' end, as with sequences of equal length, are skipped by both.
 #include <string.h>
 
+#include "row_limits.h"
 #include "series_tile.h"
 
 namespace tmp {
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
   const int lane = lane_id(), l31 = lane & 31, h8 = (lane >> 5) * 8, strip = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 32;
   const int kd = p.k.dim, vd = p.v.dim;
   const int64_t per_state = (int64_t)kd * vd;
-  const int sec0 = sec * p.section, sec1 = sec0 + p.section < p.s.n ? sec0 + p.section : p.s.n;
+  const int sec0 = sec * p.section, sec1 = section_end(sec0, p.section, p.s.n);
   int pos = sec0;
   Span sp;
   Offsets near = {0, -1};  // (nothing is found in it: filled where it is needed)

@@ -18,4 +18,7 @@ __host__ __device__ inline int window_end(int j0, int rows, int window, int n) {
   return hi < n ? (int)hi : n;
 }
 
+// The row behind the last one of the section that starts at row `first` (< n).
+__host__ __device__ inline int section_end(int first, int section, int n) { return section < n - first ? first + section : n; }
+
 }  // namespace tmp

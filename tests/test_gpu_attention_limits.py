@@ -32,3 +32,30 @@ def test_window_gradients_of_a_table_where_row_and_window_pass_32_bits():
     for name, x in zip(("dq", "dk", "dv"), ops.window_attention_grad(do, q, k, v, out, lse, 2 ** 40, offsets=off)):
         ref.check(name, x[:period], *want[name])
         assert _repeats(x, x[:period]), name
+
+
+def test_decay_attention_of_the_largest_table():
+    """One series of 2^31 - 65537 rows: what a section's start and its length add up to passes 2^31 in the last section (of
+    a walk towards the first row: at the first rows).  With a decay of exp(-1/2) four hundred rows are all that a row
+    depends on (exp(-200) of a term is nothing)."""
+    from tempo_amd import ops
+    n, period, look, far = 2 ** 31 - 65537, 6_400, 3_000, 400
+    g = torch.Generator().manual_seed(11)
+    small = [torch.randn(period, 1, 1, generator=g).to(torch.bfloat16) for _ in range(4)]
+    q, k, v, do = (x.cuda().repeat(-(-n // period), 1, 1)[:n] for x in small)
+    ld = torch.tensor([-0.5])
+    # what memory the results get holds NaN beforehand
+    junk = [torch.full((n, 1, 1), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    del junk
+    out, last = ops.decay_attention(q, k, v, ld.cuda(), scale=1.0, return_state=True)
+    grads = ops.decay_attention_grad(do, q, k, v, ld.cuda(), scale=1.0)
+    for a, b in ((0, look + far), (n - look - far, n)):
+        part = [x[a:b].cpu() for x in (q, k, v, do)]
+        want = ref.decay_reference(*part[:3], ld, [0, b - a], 1.0, dout=part[3])
+        # (a row far enough from the cut has all that it depends on)
+        behind, before = slice(0 if a == 0 else far, look + far), slice(0, look if a == 0 else look + far)
+        for name, x, rows in (("out", out, behind), ("dq", grads[0], behind), ("dk", grads[1], before), ("dv", grads[2], before)):
+            ref.check(f"{name} of rows {a}..", x[a:b][rows], want[name][0][rows], want[name][1][rows])
+    ref.check("state", last, *want["state"])
+    for x in (out, *grads):
+        assert all(bool(part.isfinite().all()) for part in x.split(1 << 28))
