@@ -14,13 +14,14 @@ device, `series_offsets(key, n_keys)` -- says where each series starts; rows bef
 offset belong to no series and get zeros.  q, k and v are [rows, heads, dim] in bfloat16 or float32 with a
 contiguous innermost dimension and any other strides (slices of one projection's output need no copy).  Both
 are differentiable in q, k and v (decay_attention in `state` too); `*_grad` are the backward passes by
-themselves, for programs that do not use autograd or capture a training step into a graph.  `*_step` add one row
-to each of some slots of kept state.  Calls do not wait for the device.
+themselves, for programs that do not use autograd or capture a training step into a graph; forward-mode
+differentiation is refused.  `*_step` add one row to each of some slots of kept state.  Calls do not wait for the device.
 """
 import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import (CacheRef, DecayAttentionArgs, DecayAttentionStepArgs, RowsRef, WindowAttentionArgs,
                    WindowAttentionStepArgs, WindowCacheWriteArgs, check, lib)
@@ -110,6 +111,14 @@ def _workspace(nbytes, device):
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 
 
+def _no_tangent(*tensors):
+    """Forward-mode differentiation: the kernels would drop the tangents without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("attention over series has no forward-mode derivative")
+
+
 def _int_arg(value, name, low):
     if isinstance(value, bool) or int(value) != value or value < low:
         raise ValueError(f"{name} must be an integer >= {low}")
@@ -167,6 +176,7 @@ def _decay_forward(q, k, v, log_decay, offsets, scale, state, return_state):
 def decay_attention_grad(dout, q, k, v, log_decay, offsets=None, scale=None, state=None, dstate=None, return_dstate=False):
     """Backward of `decay_attention`: (dq, dk, dv), and with return_dstate the gradient of `state` behind them.
     dout: gradient of out; dstate: gradient of the returned state, if that was used."""
+    _no_tangent(dout, q, k, v, log_decay, state, dstate)
     a, n_series = _decay_args(q, k, v, log_decay, offsets, scale, state)
     n, heads, dk = q.shape
     dv = v.shape[2]
@@ -210,6 +220,7 @@ def decay_attention(q, k, v, log_decay, offsets=None, scale=None, state=None, re
     scale defaults to dk ** -0.5 and must be positive.  state float32 [n_series, heads, dk, dv]: what the
     rows before this call left (None: nothing); return_state hands back the same for the call that goes on, or
     for `decay_attention_step`.  Returns out [n, heads, dv], or (out, state)."""
+    _no_tangent(q, k, v, log_decay, state)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, state, log_decay)):
         return _DecayAttention.apply(q, k, v, log_decay, offsets, scale, state, bool(return_state))
     out, last = _decay_forward(q, k, v, log_decay, offsets, scale, state, return_state)
@@ -234,6 +245,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One new row for each of some series: q, k [b, heads, dk], v [b, heads, dv]; state float32 [n_slots, heads,
     dk, dv], changed in place; slots int32 [b] (None: row i is slot i).  A row whose slot is out of range or named
     by an earlier row changes nothing and results in NaN; with slots b is at most 65536.  Returns out [b, heads, dv]."""
+    _no_tangent(q, k, v, log_decay, state)
     q = _rows_check(q, "q")
     n, heads, dk = q.shape
     k = _rows_check(k, "k", q, n, heads, dk)
@@ -285,6 +297,7 @@ def _window_forward(q, k, v, window, sinks, offsets, scale, return_lse):
 
 def window_attention_grad(dout, q, k, v, out, lse, window, sinks=0, offsets=None, scale=None):
     """Backward of `window_attention`: (dq, dk, dv) from dout and what the forward returned (out, lse)."""
+    _no_tangent(dout, q, k, v, out, lse)
     a = _window_args(q, k, v, window, sinks, offsets, scale)
     n, heads, dv = q.shape[0], q.shape[1], v.shape[2]
     dout = _rows_check(dout, "dout", q, n, heads, dv)
@@ -323,6 +336,7 @@ def window_attention(q, k, v, window, sinks=0, offsets=None, scale=None, return_
     i sees rows j <= i of its series with j > i - window, and the series' first `sinks` rows.  scale defaults to
     dk ** -0.5 and must be positive.  Returns out [n, heads, dv], with return_lse also the log of the sum of
     exponentials of each row's scores, float32 [n, heads] (-inf for rows of no series; no gradient)."""
+    _no_tangent(q, k, v)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         out, lse = _WindowAttention.apply(q, k, v, window, sinks, offsets, scale)
     else:
@@ -360,6 +374,7 @@ def window_cache_write(k, v, k_cache, v_cache, length, sinks=0, offsets=None, sl
     """Fills cache slots from whole series: after `window_attention` over k, v [n, kv_heads, dim], slot slots[s] (None:
     s) holds what `window_attention_step` needs of series s, in place of what it held.  k_cache, v_cache [n_slots,
     window + sinks, kv_heads, dim]; length int64 [n_slots]: rows seen by each slot."""
+    _no_tangent(k, v, k_cache, v_cache)
     k = _rows_check(k, "k")
     n, kv, dk = k.shape
     v = _rows_check(v, "v", k, n, kv)
@@ -381,6 +396,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
     `sinks`.  The caches' number of rows is window + sinks.  slots int32 [b] (None: row i is slot i); a row whose slot is
     out of range or named by an earlier row changes nothing and results in NaN; with slots b is at most 65536.  Returns
     out [b, heads, dv]."""
+    _no_tangent(q, k, v, k_cache, v_cache)
     q = _rows_check(q, "q")
     n, heads, dk = q.shape
     k = _rows_check(k, "k", q, n, None, dk)
