@@ -119,6 +119,12 @@ def _no_tangent(*tensors):
                 raise NotImplementedError("attention over series has no forward-mode derivative")
 
 
+def _changed(*tensors):
+    """Tells autograd that a call writes them: a backward pass that saved one of them raises instead of reading what is
+    there by then."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _int_arg(value, name, low):
     if isinstance(value, bool) or int(value) != value or value < low:
         raise ValueError(f"{name} must be an integer >= {low}")
@@ -262,6 +268,7 @@ def decay_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     a = DecayAttentionStepArgs(n=n, n_slots=state.shape[0], slots=_p(slots), type=_TYPES[q.dtype], heads=heads, dim_k=dk,
                                dim_v=dv, scale=_scale(scale, dk), log_decay=log_decay.data_ptr(), q=_ref(q), k=_ref(k),
                                v=_ref(v), out=_ref(out), state=state.data_ptr())
+    _changed(state)
     with _current(q.device):
         check(lib().tmp_decay_attention_step(C.byref(a), _stream(q.device)), "tmp_decay_attention_step")
     return out
@@ -386,6 +393,7 @@ def window_cache_write(k, v, k_cache, v_cache, length, sinks=0, offsets=None, sl
     a = WindowCacheWriteArgs(n=n, n_series=n_series, offsets=_p(offsets), n_slots=n_slots, slots=_p(slots),
                              type=_TYPES[k.dtype], kv_heads=kv, dim_k=dk, dim_v=dv, window=window, sinks=sinks, k=_ref(k),
                              v=_ref(v), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache), length=length.data_ptr())
+    _changed(k_cache, v_cache, length)
     with _current(k.device):
         check(lib().tmp_window_cache_write(C.byref(a), _stream(k.device)), "tmp_window_cache_write")
 
@@ -413,6 +421,7 @@ def window_attention_step(q, k, v, k_cache, v_cache, length, sinks=0, slots=None
                                 dim_k=dk, dim_v=dv, window=window, sinks=sinks, scale=_scale(scale, dk), q=_ref(q), k=_ref(k),
                                 v=_ref(v), out=_ref(out), k_cache=_cache_ref(k_cache), v_cache=_cache_ref(v_cache),
                                 length=length.data_ptr())
+    _changed(k_cache, v_cache, length)
     with _current(q.device):
         ws = _workspace(lib().tmp_window_attention_step_workspace_bytes(C.byref(a)), q.device)
         check(lib().tmp_window_attention_step(C.byref(a), ws.data_ptr(), ws.numel(), _stream(q.device)),

@@ -59,3 +59,41 @@ def test_decay_attention_of_the_largest_table():
     ref.check("state", last, *want["state"])
     for x in (out, *grads):
         assert all(bool(part.isfinite().all()) for part in x.split(1 << 28))
+
+
+def test_steps_tell_autograd_what_they_change():
+    """A backward pass whose saved state or rows a step has changed since raises, as with torch's own in-place operations;
+    with another state's step, and in inference mode, calls go on as ever."""
+    from tempo_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rows = lambda n=6: torch.randn(n, 2, 16, generator=g, device="cuda")  # noqa: E731
+    q, k, v = rows().requires_grad_(), rows(), rows()
+    ld = torch.tensor([-0.1, -0.2], device="cuda")
+    state, other = torch.zeros(1, 2, 16, 16, device="cuda"), torch.zeros(1, 2, 16, 16, device="cuda")
+    out = ops.decay_attention(q, k, v, ld, state=state)
+    ops.decay_attention_step(rows(1), rows(1), rows(1), ld, other)
+    out.sum().backward(retain_graph=True)
+    ops.decay_attention_step(rows(1), rows(1), rows(1), ld, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    # rows of a cache, read in place as keys and values of the whole form
+    kc, vc = rows(8).reshape(2, 4, 2, 16), rows(8).reshape(2, 4, 2, 16)
+    length = torch.tensor([4, 4], device="cuda")
+    writes = {
+        "step": lambda: ops.window_attention_step(rows(2), rows(2), rows(2), kc, vc, length),
+        "write": lambda: ops.window_cache_write(rows(4), rows(4), kc, vc, length, offsets=torch.tensor([0, 1, 4], device="cuda")),
+    }
+    for write in writes.values():
+        for keys, values in ((kc[0], rows(4)), (rows(4), vc[0])):
+            out = ops.window_attention(rows(4).requires_grad_(), keys, values, 3)
+            counted = length._version
+            write()
+            assert length._version > counted
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.sum().backward()
+    with torch.inference_mode():
+        made = torch.zeros(1, 2, 16, 16, device="cuda")
+        ops.decay_attention_step(rows(1), rows(1), rows(1), ld, made)
+        ops.decay_attention_step(rows(1), rows(1), rows(1), ld, state)
+        for write in writes.values():
+            write()
