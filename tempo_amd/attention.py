@@ -150,7 +150,7 @@ def _decay_args(q, k, v, log_decay, offsets, scale, state):
     v = _rows_check(v, "v", q, n, heads)
     dv = v.shape[2]
     _plain_check(log_decay, "log_decay", torch.float32, (heads,), q.device)
-    if log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay has no gradient: detach it")
     n_series = _offsets_check(offsets, q.device)
     if state is not None:
@@ -222,12 +222,15 @@ class _DecayAttention(torch.autograd.Function):
 def decay_attention(q, k, v, log_decay, offsets=None, scale=None, state=None, return_state=False):
     """Linear attention with a decay for each head over whole series (beside `ops.ema`).
 
-    q, k [n, heads, dk], v [n, heads, dv]; log_decay float32 [heads], <= 0 (-inf: a row sees itself alone);
+    q, k [n, heads, dk], v [n, heads, dv]; log_decay float32 [heads], <= 0 (-inf: a row sees itself alone), without a
+    gradient: detached, or under no_grad;
     scale defaults to dk ** -0.5 and must be positive.  state float32 [n_series, heads, dk, dv]: what the
     rows before this call left (None: nothing); return_state hands back the same for the call that goes on, or
     for `decay_attention_step`.  Returns out [n, heads, dv], or (out, state)."""
     _no_tangent(q, k, v, log_decay, state)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, state, log_decay)):
+        if isinstance(log_decay, torch.Tensor) and log_decay.requires_grad:  # (asked here: within forward() gradients are off)
+            raise ValueError("log_decay has no gradient: detach it")
         return _DecayAttention.apply(q, k, v, log_decay, offsets, scale, state, bool(return_state))
     out, last = _decay_forward(q, k, v, log_decay, offsets, scale, state, return_state)
     return (out, last) if return_state else out

@@ -97,3 +97,27 @@ def test_steps_tell_autograd_what_they_change():
         ops.decay_attention_step(rows(1), rows(1), rows(1), ld, state)
         for write in writes.values():
             write()
+
+
+def test_decays_held_as_a_parameter():
+    """Without gradients such a decay is as good as any; where one is wanted it is refused, at every entry."""
+    from tempo_amd import ops
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v, do = (torch.randn(40, 2, 16, generator=g, device="cuda") for _ in range(4))
+    ld = torch.nn.Parameter(torch.tensor([-0.1, -0.02], device="cuda"))
+    state = torch.zeros(40, 2, 16, 16, device="cuda")
+    with torch.no_grad():
+        assert torch.equal(ops.decay_attention(q, k, v, ld), ops.decay_attention(q, k, v, ld.detach()))
+        for a, b in zip(ops.decay_attention_grad(do, q, k, v, ld), ops.decay_attention_grad(do, q, k, v, ld.detach())):
+            assert torch.equal(a, b)
+        ops.decay_attention_step(q, k, v, ld, state)
+    for call in (lambda: ops.decay_attention(q, k, v, ld), lambda: ops.decay_attention_grad(do, q, k, v, ld),
+                 lambda: ops.decay_attention(q.clone().requires_grad_(), k, v, ld)):
+        with pytest.raises(ValueError, match="log_decay has no gradient"):
+            call()
+    with pytest.raises(ValueError, match="gradient"):
+        ops.decay_attention_step(q, k, v, ld, state)
+    # detached it trains the rest
+    leaf = q.clone().requires_grad_()
+    ops.decay_attention(leaf, k, v, ld.detach()).backward(do)
+    assert torch.equal(leaf.grad, ops.decay_attention_grad(do, q, k, v, ld.detach())[0]) and ld.grad is None
