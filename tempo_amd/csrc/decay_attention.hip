@@ -519,10 +519,12 @@ static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPl
   p.s.offsets = a->offsets; p.s.n_series = a->offsets ? a->n_series : 1; p.s.n = (int32_t)a->n;
   p.log_decay = a->log_decay;
   p.carry = d.carry + walk * d.per_walk; p.link = d.link + walk * (d.sections + 1); p.section = d.section; p.sections = d.sections;
-  // Few rows in many series: one launch, whose blocks walk the rows of their first series that lie before them once
-  // more, costs less than three (2000 rows of 100 series, 4 heads of 64: 20 us against 29 us); a single series would
-  // make the last block walk all of them.
-  p.alone = a->n <= 4096 && a->n / (p.s.n_series > 0 ? p.s.n_series : 1) <= 128;
+  // Few rows: one launch, whose blocks walk the rows of their first series that lie before them once more, costs less than
+  // three.  Lengths are known on the device only, so the bound is where one block's walk over all rows still takes no longer
+  // than the three (us of a call, one series of all rows among empty ones | series of 20 rows; one launch, three launches):
+  // bf16 4 x 64/64 512 rows 21, 21 | 13, 24, 1024 rows 37, 23 | 13, 26; 16 x 128/128 512 rows 31, 34 | 15, 33, 1024 rows
+  // 57, 39 | 15, 35; float 8 x 40/72 256 rows 27, 29 | 23, 32, 512 rows 45, 30 | 23, 33; 2 x 128/128 256 rows 44, 44 | 37, 50.
+  p.alone = a->n <= (a->type == TMP_BF16 ? 512 : 256);
   p.heads = a->heads; p.scale = a->scale; p.in_by = 1.f; p.out_by = 1.f;
   return p;
 }

@@ -121,3 +121,29 @@ def test_decays_held_as_a_parameter():
     leaf = q.clone().requires_grad_()
     ops.decay_attention(leaf, k, v, ld.detach()).backward(do)
     assert torch.equal(leaf.grad, ops.decay_attention_grad(do, q, k, v, ld.detach())[0]) and ld.grad is None
+
+
+@pytest.mark.parametrize("dtype, few", [(torch.bfloat16, 512), (torch.float32, 256)], ids=["bf16", "f32"])
+def test_one_long_series_among_empty_ones(dtype, few):
+    """Sections of a long series are walked side by side however many empty series there are besides; up to `few` rows
+    every block walks what it needs in one launch.  Either way results are the definition's."""
+    from tempo_amd import _lib, ops
+    h, dk, dv = 2, 24, 40
+    ld = torch.tensor([-0.1, -0.004])
+    for n, launches in ((few - 1, 1), (few, 1), (few + 1, 3), (1500, 3), (4096, 3)):
+        g = torch.Generator().manual_seed(n)
+        q, k, v, do = (torch.randn(n, h, d, generator=g).to(dtype) for d in (dk, dk, dv, dv))
+        off = [0] * 60 + [n] * 61
+        d, o = [x.cuda() for x in (q, k, v, do)], torch.tensor(off, device="cuda")
+        want = ref.decay_reference(q, k, v, ld, off, dk ** -0.5, dout=do)
+        _lib.profile_enable(True)
+        try:
+            _lib.profile_reset()
+            out = ops.decay_attention(*d[:3], ld.cuda(), offsets=o)
+            torch.cuda.synchronize()
+            assert len(_lib.profile_read()) == launches, n
+        finally:
+            _lib.profile_enable(False)
+        ref.check("out", out, *want["out"])
+        for name, x in zip(("dq", "dk", "dv"), ops.decay_attention_grad(d[3], *d[:3], ld.cuda(), offsets=o)):
+            ref.check(name, x, *want[name])
