@@ -22,11 +22,11 @@ constexpr int WA_TILE = 64;    // rows of a streamed tile
 constexpr int WA_THREADS = 256;
 constexpr int WA_SECTION = WA_OWN;  // query rows whose share of the sinks' gradients one block adds up
 
-// bfloat16: dS enters dq as the sum of two numbers, since its own rounding would come on top of that of do.o (of the
-// rounded out): error against 64 bits at window 1000, head size 64 1.82e-3, 2.48e-3 with one number (rounding dq itself
-// is 1.65e-3); 32768 x 16 x 64: 294 us, 250 us with one.  For dk, whose do.o are many rows', it does so up to this
-// window (11: 2.00e-3 and 2.60e-3, dk and dv there 6 % slower); beyond, one number costs less than it saves.
-constexpr int WA_FINE = 64;
+// bfloat16: dS enters dq and dk as the sum of two numbers at every window, since its own rounding would come on top of those
+// of the result and of do.o (of the rounded out).  Error against 64 bits where rounding the result alone is 1.66e-3, two
+// numbers | one: dq at window 1000, head size 64 1.82e-3 | 2.48e-3; dk 1.80e-3 | 2.44e-3, at window 70 1.75e-3 | 2.41e-3, at
+// 11 2.00e-3 | 2.60e-3.  32768 x 16 x 64, window 1000: dq 300 | 250 us, dk and dv 406 | 350 us.  The weights P enter out and
+// dv as one number (out 2.1e-3, dv 2.3e-3): a sum of rounded positive terms, whose second product would cost as much again.
 
 struct WindowParams {
   Series s;
@@ -633,7 +633,7 @@ __global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkd
       } else {
         add_rows<T, D>(dv, dt, u * 32, s);
         add_rows<T, D>(dk, qt, u * 32, dp);
-        if (sizeof(T) == 2 && p.window <= WA_FINE) add_rows<T, D>(dk, qt, u * 32, left_over<T>(dp));
+        if (sizeof(T) == 2) add_rows<T, D>(dk, qt, u * 32, left_over<T>(dp));
       }
     }
   }

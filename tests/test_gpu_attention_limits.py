@@ -147,3 +147,25 @@ def test_one_long_series_among_empty_ones(dtype, few):
         ref.check("out", out, *want["out"])
         for name, x in zip(("dq", "dk", "dv"), ops.decay_attention_grad(d[3], *d[:3], ld.cuda(), offsets=o)):
             ref.check(name, x, *want[name])
+
+
+@pytest.mark.parametrize("d, heads, kv, sinks", [(32, 2, 2, 0), (64, 4, 2, 0), (128, 4, 2, 4)])
+@pytest.mark.parametrize("window", [60, 64, 65, 70, 600])
+def test_errors_of_bfloat16_training_do_not_depend_on_the_window(window, d, heads, kv, sinks):
+    """Root mean square errors against 64 bits, in units of what rounding the exact result once gives.  Independent roundings
+    add in squares: the result alone is 1, one more of the same size (an operand of a product that is rounded once, as
+    the weights are for out and dv) sqrt(2), two more sqrt(3).  dS is not rounded to eight bits anywhere, so that dq and
+    dk have the result's rounding and, smaller than that over sixty rows, that of out within do.o."""
+    from tempo_amd import ops
+    n = 1500
+    q, k, v, do = (torch.randn(n, h, d, generator=torch.Generator().manual_seed(d + i)).bfloat16()
+                   for i, h in enumerate((heads, kv, kv, heads)))
+    off = [0, 700, n]
+    want = ref.window_reference(q, k, v, do, off, window, sinks, d ** -0.5)
+    a, o = [x.cuda() for x in (q, k, v, do)], torch.tensor(off, device="cuda")
+    out, lse = ops.window_attention(*a[:3], window, sinks=sinks, offsets=o, return_lse=True)
+    got = (out, *ops.window_attention_grad(a[3], *a[:3], out, lse, window, sinks=sinks, offsets=o))
+    for name, x, most in zip(("out", "dq", "dk", "dv"), got, (1.5, 1.2, 1.2, 1.5)):
+        exact = want[name][0]
+        alone = float((exact.bfloat16().double() - exact).norm())
+        assert float((x.cpu().double() - exact).norm()) < most * alone, name
