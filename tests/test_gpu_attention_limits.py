@@ -169,3 +169,113 @@ def test_errors_of_bfloat16_training_do_not_depend_on_the_window(window, d, head
         exact = want[name][0]
         alone = float((exact.bfloat16().double() - exact).norm())
         assert float((x.cpu().double() - exact).norm()) < most * alone, name
+
+
+def _recurrence(q, k, v, ld, off, scale, state, do=None, dstate=None):
+    """The definition row by row in 64 bits: {name: (value, sum of magnitudes)} of out, state, dq, dk, dv, dstate."""
+    n, h, dk = q.shape
+    lam = torch.exp(ld.double())[:, None, None]
+    res = {}
+    for which, of in (("value", lambda x: x), ("size", torch.abs)):
+        Q, K, V, S0 = (of(x.double()) for x in (q, k, v, state))
+        out, last = torch.zeros(n, h, v.shape[2], dtype=torch.float64), torch.zeros_like(S0)
+        dq, dk_, dv_ = torch.zeros_like(Q), torch.zeros_like(K), torch.zeros_like(V)
+        ds = torch.zeros_like(S0)
+        for s in range(len(off) - 1):
+            S = S0[s]
+            for i in range(off[s], off[s + 1]):
+                S = lam * S + K[i, :, :, None] * V[i, :, None, :]
+                out[i] = (Q[i, :, :, None] * S).sum(1) * scale
+                if do is not None:
+                    dq[i] = (S * of(do[i].double())[:, None, :]).sum(2) * scale
+            last[s] = S
+            if do is None:
+                continue
+            G = of(dstate[s].double())  # dG/dS behind row i: what the state there is worth
+            for i in range(off[s + 1] - 1, off[s] - 1, -1):
+                G = G + scale * Q[i, :, :, None] * of(do[i].double())[:, None, :]
+                dk_[i] = (G * V[i, :, None, :]).sum(2)
+                dv_[i] = (G * K[i, :, :, None]).sum(1)
+                G = lam * G
+            ds[s] = G
+        res[which] = dict(out=out, state=last, dq=dq, dk=dk_, dv=dv_, dstate=ds)
+    return {name: (res["value"][name], res["size"][name]) for name in res["value"]}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_states_strung_together_over_several_sweeps(dtype):
+    """40 000 rows of one head make 625 sections, of which a sweep of the scan takes 256; one series reaches over 560 of
+    them, slowly fading, with a state before it and a gradient of the one behind it."""
+    from tempo_amd import ops
+    off, h, dk, dv, scale = [0, 1_900, 37_900, 37_900, 40_000], 1, 16, 12, 0.25
+    n = off[-1]
+    g = torch.Generator().manual_seed(17)
+    q, k, v, do = (torch.randn(n, h, d, generator=g).to(dtype) for d in (dk, dk, dv, dv))
+    state, dstate = (torch.randn(4, h, dk, dv, generator=g) for _ in range(2))
+    ld = torch.tensor([-2e-5])
+    want = _recurrence(q, k, v, ld, off, scale, state, do, dstate)
+    a, o = [x.cuda() for x in (q, k, v, do)], torch.tensor(off, device="cuda")
+    out, last = ops.decay_attention(*a[:3], ld.cuda(), offsets=o, scale=scale, state=state.cuda(), return_state=True)
+    grads = ops.decay_attention_grad(a[3], *a[:3], ld.cuda(), offsets=o, scale=scale, state=state.cuda(), dstate=dstate.cuda(),
+                                     return_dstate=True)
+    got = dict(zip(("out", "state", "dq", "dk", "dv", "dstate"), (out, last, *grads)))
+    # rows in parts of 32, sections of 64, 625 sections: no term passes through more sums than these; powers of the decay as
+    # in the definition's bounds; bfloat16 terms are rounded once, those of a state to 2^-17
+    u = ref.half_step(dtype)
+    sums = ref.gamma(32 + 64 + 2 * 625 + dk) + 8 * ref.E32 + 90 * 2.0 ** -22
+    term = u + 2.0 ** -17 if dtype != torch.float32 else 2 * ref.E32
+    for name, x in got.items():
+        exact, size = want[name]
+        fine = name in ("state", "dstate")
+        ref.check(name, x, exact, (0 if fine else u * exact.abs()) + (sums + (0 if fine else term)) * size)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_gradients_that_depend_on_a_value_that_is_not_finite(dtype, bad):
+    """One bad element of an input in turn.  Where a gradient is a sum that has it, or a weight made of it, as a term, the
+    gradient is not finite: of the window's, dq of the rows whose weights it makes, dk and dv of the keys that these see, the
+    bad element of dv for dout; of the decay's, every sum with it as a factor.  (A key whose score is minus infinity has the
+    weight zero: the row's other weights are as finite as ever, and zero times the key is not.)"""
+    from tempo_amd import ops
+    lens, window, sinks, h, d, head, e = [60, 300, 45], 20, 2, 2, 32, 1, 7
+    off = [0, 60, 360, 405]
+    n = off[-1]
+    o = torch.tensor(off, device="cuda")
+    g = torch.Generator().manual_seed(78)
+    clean = [torch.randn(n, h, d, generator=g).to(dtype) for _ in range(4)]
+    ld = torch.tensor([-0.1, -0.02]).cuda()
+    seen = ref.window_mask(n, off, window, sinks)
+    sid, pos = ref.series_of(n, off)
+    past = (sid[:, None] == sid[None]) & (pos[None] <= pos[:, None])
+    none = torch.zeros(n, dtype=torch.bool)
+    for which, row in ((0, 100), (0, 61), (1, 60), (1, 61), (1, 200), (2, 60), (2, 201), (3, 150), (3, 62)):
+        ts = [x.clone() for x in clean]
+        ts[which][row, head, e] = bad
+        q, k, v, do = (x.cuda() for x in ts)
+        out, lse = ops.window_attention(q, k, v, window, sinks=sinks, offsets=o, return_lse=True)
+        grads = [x.float().cpu()[:, head] for x in ops.window_attention_grad(do, q, k, v, out, lse, window, sinks=sinks, offsets=o)]
+        at = none.clone()
+        at[row] = True
+        rows = at if which in (0, 3) else seen[:, row]  # query rows with a weight, or a gradient of one, that is not finite
+        if which == 1:
+            assert not bool(grads[0][rows][:, e].isfinite().any()), (which, row)
+            rows = rows & ~(ts[0][:, head, e].float() * bad == -float("inf"))
+        keys = seen[rows].any(0)
+        for i, (name, x) in enumerate(zip(("dq", "dk", "dv"), grads)):
+            touched = rows if i == 0 else keys
+            if which == 2 and i == 2:
+                continue  # (weights do not depend on v: dv stays finite)
+            part = x[touched][:, e] if i == 2 and which == 3 else x[touched]
+            assert not bool(part.isfinite().any()), (name, which, row)
+        # S_i of rows behind, G_i of rows before: element e is a row or a column of them
+        grads = [x.float().cpu()[:, head] for x in ops.decay_attention_grad(do, q, k, v, ld, offsets=o)]
+        behind, before = past[:, row], past[row]
+        bad_part = {  # input: (gradient, rows, elements)
+            0: [(1, before, [e]), (2, before, slice(None))],
+            1: [(0, behind, [e]), (2, at, slice(None))],
+            2: [(0, behind, slice(None)), (1, at, slice(None))],
+            3: [(0, at, slice(None)), (1, before, slice(None)), (2, before, [e])],
+        }[which]
+        for i, rows, elems in bad_part:
+            assert not bool(grads[i][rows][:, elems].isfinite().any()), ("decay", i, which, row)
