@@ -11,7 +11,8 @@
 // Backward (G_i = scale q_i do_i^T + lambda G_{i+1}, the same recurrence from the last row to the first):
 //   dq_i = scale S_i do_i     dk_i = G_i v_i     dv_i = G_i^T k_i     dS_0 = lambda G_1
 // are three walks of the same kernel with the roles of the rows exchanged; the walks towards the first
-// row keep Y = lambda G, so that o takes lambda^r of it and the update lambda^{len-s}.
+// row keep Y = lambda G, so that o takes lambda^r of it and the update lambda^{len-s}.  The factor `scale` enters S's
+// results and G itself: states are what the caller gives and gets, whatever the scale.
 //
 // The table is cut into sections of rows that are walked side by side.  Where a series reaches over a
 // section's start, a first launch walks each section for the state it adds (keys and values only) and a
@@ -38,7 +39,7 @@ struct DecayParams {
   int32_t heads, section, sections;
   int32_t alone;  // a section's block walks a series that reaches over its start from that series' first row
   int32_t reverse, transposed;  // walk from the last row; states lie as [dv][dk] of this walk's roles
-  float scale, in_by, out_by;   // of rows, and of states read and written
+  float scale;
 };
 
 // Walks that are launched together, one to each blockIdx.y: the backward pass's three have the same sections.
@@ -68,7 +69,7 @@ __device__ inline uint32_t state_at(int lane, int t, int x, int kd, int vd, bool
   const int dk = 32 * t + 16 * (x >> 3) + (lane >> 5) * 8 + (x & 7), dv = (threadIdx.x >> 6) * 32 + pi_of(lane & 31);
   return dk < kd && dv < vd ? (transposed ? dv * kd + dk : dk * vd + dv) * 4 : kOutside;
 }
-template <int NT> __device__ inline void state_load(f32x16 (&st)[NT], const float *p, int kd, int vd, bool transposed, float by) {
+template <int NT> __device__ inline void state_load(f32x16 (&st)[NT], const float *p, int kd, int vd, bool transposed) {
   const Buffer b = buffer_of(p, kd * vd * 4);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -76,18 +77,24 @@ template <int NT> __device__ inline void state_load(f32x16 (&st)[NT], const floa
     asm volatile("" : "+v"(lane));  // (keeps the offsets from being held in registers over the walk)
 #pragma unroll
     for (int x = 0; x < 16; ++x)
-      st[t][x] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, state_at(lane, t, x, kd, vd, transposed), 0, 0)) * by;
+      st[t][x] = __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, state_at(lane, t, x, kd, vd, transposed), 0, 0));
   }
+  // They are waited for here: left to their first use, which lies in the walk's loop, the wait would stand there and be one
+  // for the next tile's rows too, part after part (131072 x 16 x 128: 13 % of the walk).
+#pragma unroll
+  for (int t = 0; t < NT; ++t) asm volatile("" : "+v"(st[t]));
 }
-template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], float *p, int kd, int vd, bool transposed, float by) {
+template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], float *p, int kd, int vd, bool transposed) {
   const Buffer b = buffer_of(p, kd * vd * 4);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     int lane = lane_id();
     asm volatile("" : "+v"(lane));
 #pragma unroll
-    for (int x = 0; x < 16; ++x)
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, st[t][x] * by), b, state_at(lane, t, x, kd, vd, transposed), 0, 0);
+    for (int x = 0; x < 16; ++x) {
+      const float y = st[t][x];  // (a bit cast of the vector's element itself is one of its first element)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), b, state_at(lane, t, x, kd, vd, transposed), 0, 0);
+    }
   }
 }
 
@@ -167,12 +174,13 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
   if (threadIdx.x < 2) flag[threadIdx.x] = 0;
   const float ld = p.log_decay[head] * kLog2e;
   const int post = p.reverse ? 1 : 0;
+  const float scale_out = p.reverse ? 1.f : p.scale, scale_in = p.reverse ? p.scale : 1.f;  // of states' results, of what is added to them
   // Decays that every whole part shares.  TABLE: they lie in LDS, four to a lane at a time, and leave 32 registers to
   // the state (131072 x 16 x 128 bf16: 517 us with two waves a SIMD, 666 us with one); else in registers, which answer
   // sooner (2000 x 4 x 64: 19 us against 23 us).
   constexpr bool TABLE = DK * sizeof(T) >= 256;
   __shared__ f32x4 within[TABLE ? 4 : 1][64];  // scale lambda^{i-j} of a part's rows i and j <= i
-  __shared__ f32x4 behind[2][4];               // lambda^{SUB-1-s+post}
+  __shared__ f32x4 behind[2][4];               // lambda^{SUB-1-s+post}, with the scale towards the first row
   float wd[16], w_all[SUB / 2];
   if (TABLE) {
     for (int g = threadIdx.x >> 6; g < 4; g += THREADS / 64) {
@@ -186,17 +194,17 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
     }
     if (threadIdx.x < 32) {
       const int g = (threadIdx.x >> 2) & 3, j = 16 * (g >> 1) + 8 * (threadIdx.x >> 4) + 4 * (g & 1) + (threadIdx.x & 3);
-      ((float *)behind)[threadIdx.x] = power(ld, SUB - 1 - j + post);
+      ((float *)behind)[threadIdx.x] = scale_in * power(ld, SUB - 1 - j + post);
     }
   } else {
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       const int j = 16 * (x >> 3) + h8 + (x & 7);
       wd[x] = OUT && j <= l31 ? p.scale * power(ld, l31 - j) : 0.f;
-      w_all[x] = power(ld, SUB - 1 - j + post);
+      w_all[x] = scale_in * power(ld, SUB - 1 - j + post);
     }
   }
-  const float into = p.scale * power(ld, l31 + 1 - post), fade_all = power(ld, SUB);
+  const float into = scale_out * power(ld, l31 + 1 - post), fade_all = power(ld, SUB);
   f32x16 st[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) st[t] = zero16();
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
                           : p.state_in ? p.state_in + ((int64_t)sp.index * p.heads + head) * per_state : nullptr;
       if (from) {
         const bool own = sp.start < pos;  // a carry lies as this walk left it
-        state_load(st, from, kd, vd, !own && p.transposed, own ? 1.f : p.in_by);
+        state_load(st, from, kd, vd, !own && p.transposed);
       } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t) st[t] = zero16();
@@ -324,7 +332,7 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int left = rows - 1 - (16 * b + h8 + e);
-            w[e] = left >= 0 ? power(ld, left + post) : 0.f;
+            w[e] = left >= 0 ? scale_in * power(ld, left + post) : 0.f;
           }
           state_add<DK, EXACT>(st, kt, r0 + 16 * b, w, col_frag<DV>(vt, r0 + 16 * b, strip, l), l);
         }
@@ -338,14 +346,14 @@ __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(De
       }
     }
     if (OUT && ends && sp.index >= 0 && p.state_out)
-      state_store(st, p.state_out + ((int64_t)sp.index * p.heads + head) * per_state, kd, vd, p.transposed, p.out_by);
+      state_store(st, p.state_out + ((int64_t)sp.index * p.heads + head) * per_state, kd, vd, p.transposed);
     fresh = ends;
     if (next >= sec1) break;
     pos = next;
     len = nlen;
     sp = nsp;
   }
-  if (!OUT) state_store(st, p.carry + ((int64_t)(sec + 1) * p.heads + head) * per_state, kd, vd, false, 1.f);
+  if (!OUT) state_store(st, p.carry + ((int64_t)(sec + 1) * p.heads + head) * per_state, kd, vd, false);
 }
 
 // carry[s] holds what section s - 1 adds; link[s] = 2: all of that section is the one series that goes on
@@ -525,7 +533,7 @@ static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPl
   // bf16 4 x 64/64 512 rows 21, 21 | 13, 24, 1024 rows 37, 23 | 13, 26; 16 x 128/128 512 rows 31, 34 | 15, 33, 1024 rows
   // 57, 39 | 15, 35; float 8 x 40/72 256 rows 27, 29 | 23, 32, 512 rows 45, 30 | 23, 33; 2 x 128/128 256 rows 44, 44 | 37, 50.
   p.alone = a->n <= (a->type == TMP_BF16 ? 512 : 256);
-  p.heads = a->heads; p.scale = a->scale; p.in_by = 1.f; p.out_by = 1.f;
+  p.heads = a->heads; p.scale = a->scale;
   return p;
 }
 
@@ -602,9 +610,7 @@ extern "C" int tmp_decay_attention_grad(const tmp_decay_attention_args *a, void 
   p0.state_in = a->state_in; p0.transposed = 1;
   p1.q = v; p1.k = o; p1.v = q; p1.out = dk; p1.transposed = 1;
   p2.q = k; p2.k = q; p2.v = o; p2.out = dv;
-  for (int i = 1; i < 3; ++i) {
-    w.p[i].reverse = 1; w.p[i].state_in = a->dstate_out; w.p[i].in_by = 1.f / a->scale; w.p[i].out_by = a->scale;
-  }
+  for (int i = 1; i < 3; ++i) { w.p[i].reverse = 1; w.p[i].state_in = a->dstate_out; }
   p2.state_out = a->dstate_in;
   if (a->n > 0) {
     const bool one = !p2.state_out && padded_dim(a->dim_k) == padded_dim(a->dim_v);

@@ -279,3 +279,27 @@ def test_gradients_that_depend_on_a_value_that_is_not_finite(dtype, bad):
         }[which]
         for i, rows, elems in bad_part:
             assert not bool(grads[i][rows][:, elems].isfinite().any()), ("decay", i, which, row)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("scale", [1e-39, 2.0 ** -100, 1e-3, 1e20])
+def test_gradients_of_states_at_every_scale(scale, dtype):
+    """The gradient of a returned state passes the backward walk as it is: a scale that is small, or no normal number, does
+    not make it overflow on its way."""
+    from tempo_amd import ops
+    off, h, dk, dv = [0, 40, 40, 400], 2, 24, 40
+    n = off[-1]
+    g = torch.Generator().manual_seed(19)
+    q, k, v, do = (torch.randn(n, h, d, generator=g).to(dtype) for d in (dk, dk, dv, dv))
+    state, dstate = (torch.randn(3, h, dk, dv, generator=g) for _ in range(2))
+    dstate *= 2.0 ** 40
+    ld = torch.tensor([-0.1, -0.004])
+    scale = float(torch.tensor(scale))  # (as the kernels take it)
+    want = ref.decay_reference(q, k, v, ld, off, scale, state, do, dstate)
+    a, o = [x.cuda() for x in (q, k, v, do)], torch.tensor(off, device="cuda")
+    grads = ops.decay_attention_grad(a[3], *a[:3], ld.cuda(), offsets=o, scale=scale, state=state.cuda(), dstate=dstate.cuda(),
+                                     return_dstate=True)
+    for name, x in zip(("dk", "dv", "dstate"), grads[1:]):
+        ref.check(name, x, *want[name])
+    if scale >= 2.0 ** -100:  # (below, products of two small factors are no normal numbers)
+        ref.check("dq", grads[0], *want["dq"])
