@@ -370,7 +370,8 @@ static int step_check_common(int64_t n, int32_t n_slots, const int32_t *slots, i
   TMP_REQUIRE(!slots || n <= TMP_MAX_SLOT_ROWS, TMP_EUNSUPPORTED, "%s: at most %d rows with slots", what, TMP_MAX_SLOT_ROWS);
   TMP_REQUIRE(n_slots >= 0 && (slots || n <= n_slots), TMP_EINVAL, "%s: more rows than slots", what);
   TMP_REQUIRE(type == TMP_BF16 || type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
-  TMP_REQUIRE(heads > 0 && heads <= 65536 && n * heads < (1ll << 31), TMP_EINVAL, "%s: bad number of heads", what);
+  TMP_REQUIRE(heads > 0 && heads <= 65536, TMP_EINVAL, "%s: heads must be in [1, 65536]", what);
+  TMP_REQUIRE(n * heads <= kMostBlocks, TMP_EUNSUPPORTED, "%s: too many rows x heads, at most 2^24 - 8", what);
   TMP_REQUIRE(dk > 0 && dv > 0, TMP_EINVAL, "%s: head sizes must be positive", what);
   TMP_REQUIRE(dk <= TMP_MAX_HEAD_DIM && dv <= TMP_MAX_HEAD_DIM, TMP_EUNSUPPORTED, "%s: head sizes are limited to %d", what,
               TMP_MAX_HEAD_DIM);
@@ -388,7 +389,8 @@ static int window_step_check(const tmp_window_attention_step_args *a, const char
 }
 
 // Rows of the cache that one wave takes: all of them once rows x heads give every compute unit eight
-// waves (two a SIMD), else such a share that they do, 32 at least.
+// waves (two a SIMD), else such a share that they do, 32 at least.  (Splits add at most WS_MOST_SPLITS waves to one for each
+// row and head.)
 static void window_step_split(const tmp_window_attention_step_args *a, int *splits, int *chunk) {
   const int64_t cap = (int64_t)a->window + a->sinks, group = a->heads / a->kv_heads;
   const int64_t units = (a->n > 0 ? a->n : 1) * a->kv_heads * ((group + 31) / 32);
@@ -479,8 +481,6 @@ extern "C" int tmp_window_attention_step(const tmp_window_attention_step_args *a
   p.n = (int32_t)a->n; p.n_slots = a->n_slots; p.heads = a->heads; p.kv_heads = a->kv_heads;
   p.window = a->window; p.sinks = a->sinks; p.scale = a->scale;
   window_step_split(a, &p.splits, &p.chunk);
-  const int64_t units = a->n * a->kv_heads * ((a->heads / a->kv_heads + 31) / 32) * p.splits;
-  TMP_REQUIRE(units < (1ll << 31) - 8, TMP_EUNSUPPORTED, "%s: too many rows x heads", what);
   hipStream_t st = (hipStream_t)stream;
   const int d = padded_dim(a->dim_k > a->dim_v ? a->dim_k : a->dim_v);
   TMP_BY_FORM(window_step, a->type, d, p.kc.vec && p.vc.vec, p, st);
@@ -512,7 +512,8 @@ extern "C" int tmp_window_cache_write(const tmp_window_cache_write_args *a, void
   p.length = a->length; p.slots = a->slots; p.n_slots = a->n_slots; p.kv_heads = a->kv_heads;
   p.window = a->window; p.sinks = a->sinks;
   p.chunks = (p.window + p.sinks + CW_ROWS - 1) / CW_ROWS;
-  TMP_REQUIRE((int64_t)p.chunks * a->n_series < (1ll << 31), TMP_EUNSUPPORTED, "%s: too many series x rows", what);
+  TMP_REQUIRE((int64_t)p.chunks * a->n_series <= kMostBlocks, TMP_EUNSUPPORTED,
+              "%s: too many series x rows of a cache, at most 2^24 - 8 times %d", what, CW_ROWS);
   const dim3 grid((unsigned)((int64_t)p.chunks * a->n_series)), block(256);
   hipStream_t st = (hipStream_t)stream;
   ProfScope ps("window_cache_write_kernel", st);

@@ -409,15 +409,16 @@ __global__ __launch_bounds__(DA_SCAN_WAVES * 64) void decay_scan_kernel(DecayWal
 }
 
 // A series without rows keeps its state.
-__global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t per_series) {
-  const int s = blockIdx.x;
-  int64_t a = 0, b = p.s.n;
-  if (p.s.offsets) { a = p.s.offsets[s]; b = p.s.offsets[s + 1]; }
-  if (b > p.s.n) b = p.s.n;
-  if (a < 0) a = 0;
-  if (a < b) return;
-  for (int64_t e = threadIdx.x; e < per_series; e += 256)
-    p.state_out[s * per_series + e] = p.state_in ? p.state_in[s * per_series + e] : 0.f;
+__global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t n_series, int64_t per_series) {
+  for (int64_t s = blockIdx.x; s < n_series; s += gridDim.x) {
+    int64_t a = 0, b = p.s.n;
+    if (p.s.offsets) { a = p.s.offsets[s]; b = p.s.offsets[s + 1]; }
+    if (b > p.s.n) b = p.s.n;
+    if (a < 0) a = 0;
+    if (a < b) continue;
+    for (int64_t e = threadIdx.x; e < per_series; e += 256)
+      p.state_out[s * per_series + e] = p.state_in ? p.state_in[s * per_series + e] : 0.f;
+  }
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -539,7 +540,7 @@ static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPl
 
 static int decay_empty(const DecayParams &p, int64_t n_series, int64_t per_series, hipStream_t st) {
   if (p.state_out && n_series > 0)
-    TMP_LAUNCH(decay_empty_kernel, dim3((unsigned)n_series), dim3(256), st, p, per_series);
+    TMP_LAUNCH(decay_empty_kernel, dim3((unsigned)(n_series < 65536 ? n_series : 65536)), dim3(256), st, p, n_series, per_series);
   return TMP_OK;
 }
 

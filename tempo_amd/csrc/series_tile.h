@@ -471,6 +471,10 @@ inline bool rows_of(const tmp_rows &r, int64_t n, int dim, int bytes, Rows *o) {
   TMP_REQUIRE(rows_of(ref, n, dim, bytes, to), TMP_EUNSUPPORTED,                                               \
               "%s: the row stride of " #ref " must be at least its head size and below 2^22 elements, its pointer aligned", what)
 
+// A launch has fewer than 2^32 threads, so that one of blocks of 256 has fewer blocks than this (rounded down to eight,
+// for grids that are a multiple of it).
+constexpr int64_t kMostBlocks = (1 << 24) - 8;
+
 // fn<T, D, VEC>(...) for a type, a padded head size and an access width.
 #define TMP_BY_DIM(fn, T, d, VEC, ...)              \
   do {                                              \

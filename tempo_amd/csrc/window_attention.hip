@@ -713,7 +713,8 @@ static int window_check(const tmp_window_attention_args *a, const char *what, bo
   TMP_REQUIRE(a->scale > 0.f && a->scale < INFINITY, TMP_EINVAL, "%s: scale must be positive and finite", what);
   TMP_REQUIRE(a->sinks >= 0, TMP_EINVAL, "%s: sinks must be >= 0", what);
   TMP_REQUIRE(a->sinks <= TMP_MAX_SINKS, TMP_EUNSUPPORTED, "%s: at most %d sinks", what, TMP_MAX_SINKS);
-  TMP_REQUIRE((a->n + WA_OWN - 1) / WA_OWN * a->heads < (1ll << 31) - 64, TMP_EUNSUPPORTED, "%s: too many rows x heads", what);
+  TMP_REQUIRE((a->n + WA_OWN - 1) / WA_OWN * a->heads <= kMostBlocks, TMP_EUNSUPPORTED,
+              "%s: too many rows x heads, at most 2^24 - 8 times %d", what, WA_OWN);
   if (a->n == 0) return TMP_OK;
   TMP_REQUIRE(a->q.p && a->k.p && a->v.p && a->out.p, TMP_EINVAL, "%s: null pointer", what);
   if (grad)

@@ -39,3 +39,40 @@ def test_forward_mode_is_refused():
         for call in _calls(**plain).values():
             with pytest.raises(TypeError, match="no CPU path"):
                 call()
+
+
+def _args(cls, **kw):
+    a = cls()
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_more_than_a_launch_holds_is_refused():
+    """Fewer than 2^32 threads fit a launch: what would need more is refused before the first one, so that no call ends
+    half done."""
+    import ctypes as C
+    from tempo_amd import _lib
+    h = _lib.lib()
+    rows = _lib.RowsRef(4096, 64, 16)
+    most = (1 << 24) - 8
+    a = dict(n=2 ** 31 - 65537, n_series=1, type=0, heads=2, kv_heads=2, dim_k=16, dim_v=16, window=5, sinks=1, scale=0.25, q=rows,
+             k=rows, v=rows, out=rows, dout=rows, dq=rows, dk=rows, dv=rows, lse=4096)
+    a = _args(_lib.WindowAttentionArgs, **a)
+    assert h.tmp_window_attention(C.byref(a), None) == -4 and b"rows x heads" in h.tmp_last_error()
+    assert h.tmp_window_attention_grad(C.byref(a), None, 0, None) == -4 and b"rows x heads" in h.tmp_last_error()
+    assert h.tmp_window_attention_grad_workspace_bytes(C.byref(a)) == 0
+    a.heads = a.kv_heads = 1  # the largest table of one head fits
+    assert h.tmp_window_attention_grad_workspace_bytes(C.byref(a)) > 0
+    for n, heads in ((most // 8 + 1, 8), (1 << 24, 1), (2 ** 15, 512)):
+        a = _args(_lib.DecayAttentionStepArgs, n=n, n_slots=n, type=0, heads=heads, dim_k=16, dim_v=16, scale=1.0, log_decay=4096,
+                  q=rows, k=rows, v=rows, out=rows, state=4096)
+        assert h.tmp_decay_attention_step(C.byref(a), None) == -4 and b"rows x heads" in h.tmp_last_error()
+        cache = _lib.CacheRef(4096, 640, 64, 16)
+        a = _args(_lib.WindowAttentionStepArgs, n=n, n_slots=n, type=0, heads=heads, kv_heads=heads, dim_k=16, dim_v=16, window=8,
+                  sinks=1, scale=1.0, q=rows, k=rows, v=rows, out=rows, k_cache=cache, v_cache=cache, length=4096)
+        assert h.tmp_window_attention_step(C.byref(a), None, 0, None) == -4 and b"rows x heads" in h.tmp_last_error()
+        assert h.tmp_window_attention_step_workspace_bytes(C.byref(a)) == 0
+    a = _args(_lib.WindowCacheWriteArgs, n=100, n_series=600_000, offsets=4096, n_slots=600_000, type=0, kv_heads=1, dim_k=16,
+              dim_v=16, window=1000, sinks=0, k=rows, v=rows, k_cache=cache, v_cache=cache, length=4096)
+    assert h.tmp_window_cache_write(C.byref(a), None) == -4 and b"series x rows" in h.tmp_last_error()

@@ -303,3 +303,26 @@ def test_gradients_of_states_at_every_scale(scale, dtype):
         ref.check(name, x, *want[name])
     if scale >= 2.0 ** -100:  # (below, products of two small factors are no normal numbers)
         ref.check("dq", grads[0], *want["dq"])
+
+
+def test_more_series_than_a_launch_has_blocks():
+    """States of 2^24 + 100 series, nearly all of them without rows: each keeps its own, or zeros without one."""
+    from tempo_amd import ops
+    ns, h, d = 2 ** 24 + 100, 1, 2
+    counts = torch.zeros(ns, dtype=torch.int64, device="cuda")
+    full = torch.tensor([0, 5, 65_535, 65_536, 2 ** 24 - 1, 2 ** 24, ns - 1], device="cuda")
+    counts[full] = 3
+    off = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    n = int(off[-1])
+    g = torch.Generator(device="cuda").manual_seed(23)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda") for _ in range(3))
+    ld = torch.tensor([-0.5], device="cuda")
+    state = torch.randn(ns, h, d, d, generator=g, device="cuda")
+    empty = torch.ones(ns, dtype=torch.bool, device="cuda")
+    empty[full] = False
+    _, last = ops.decay_attention(q, k, v, ld, offsets=off, state=state, return_state=True)
+    assert torch.equal(last[empty], state[empty])
+    small = torch.arange(0, n + 1, 3, device="cuda")
+    assert torch.equal(last[full], ops.decay_attention(q, k, v, ld, offsets=small, state=state[full].contiguous(), return_state=True)[1])
+    _, last = ops.decay_attention(q, k, v, ld, offsets=off, return_state=True)
+    assert not bool(last[empty].any())
