@@ -493,7 +493,7 @@ extern "C" int tmp_window_cache_write(const tmp_window_cache_write_args *a, void
   const char *what = "tmp_window_cache_write";
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_REQUIRE(a->n >= 0 && a->n < (1ll << 31) - 65536, TMP_EINVAL, "%s: row count must be in [0, 2^31 - 65536)", what);
-  TMP_REQUIRE(a->n_series >= 0 && (a->offsets || a->n_series <= 1), TMP_EINVAL, "%s: bad series", what);
+  TMP_SERIES(what, a);
   TMP_TRY(step_check_common(a->n_series, a->n_slots, a->slots, a->type, a->kv_heads, a->dim_k, a->dim_v, what));
   TMP_REQUIRE(a->window >= 1 && a->window < (1 << 30), TMP_EINVAL, "%s: window must be in [1, 2^30)", what);
   TMP_REQUIRE(a->sinks >= 0, TMP_EINVAL, "%s: sinks must be >= 0", what);

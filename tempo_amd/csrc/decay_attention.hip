@@ -454,7 +454,7 @@ static void decay_plan(const tmp_decay_attention_args *a, int walks, Workspace &
 static int decay_check(const tmp_decay_attention_args *a, const char *what, bool grad) {
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_REQUIRE(a->n >= 0 && a->n < (1ll << 31) - 65536, TMP_EINVAL, "%s: row count must be in [0, 2^31 - 65536)", what);
-  TMP_REQUIRE(a->n_series >= 0 && (a->offsets || a->n_series <= 1), TMP_EINVAL, "%s: bad series", what);
+  TMP_SERIES(what, a);
   TMP_REQUIRE(a->type == TMP_BF16 || a->type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
   TMP_REQUIRE(a->heads > 0 && a->heads <= 65536, TMP_EINVAL, "%s: heads must be in [1, 65536]", what);
   TMP_REQUIRE(a->dim_k > 0 && a->dim_v > 0, TMP_EINVAL, "%s: head sizes must be positive", what);
@@ -525,7 +525,7 @@ static void decay_run(const DecayWalks &w, int walks, int type, hipStream_t st) 
 static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d, int walk) {
   DecayParams p;
   memset(&p, 0, sizeof(p));
-  p.s.offsets = a->offsets; p.s.n_series = a->offsets ? a->n_series : 1; p.s.n = (int32_t)a->n;
+  p.s.offsets = a->offsets; p.s.n_series = a->n_series; p.s.n = (int32_t)a->n;
   p.log_decay = a->log_decay;
   p.carry = d.carry + walk * d.per_walk; p.link = d.link + walk * (d.sections + 1); p.section = d.section; p.sections = d.sections;
   // Few rows: one launch, whose blocks walk the rows of their first series that lie before them once more, costs less than

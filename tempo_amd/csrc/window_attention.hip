@@ -702,7 +702,7 @@ __global__ __launch_bounds__(256) void sink_sum_kernel(WindowParams p) {
 static int window_check(const tmp_window_attention_args *a, const char *what, bool grad) {
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_REQUIRE(a->n >= 0 && a->n < (1ll << 31) - 65536, TMP_EINVAL, "%s: row count must be in [0, 2^31 - 65536)", what);
-  TMP_REQUIRE(a->n_series >= 0 && (a->offsets || a->n_series <= 1), TMP_EINVAL, "%s: bad series", what);
+  TMP_SERIES(what, a);
   TMP_REQUIRE(a->type == TMP_BF16 || a->type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
   TMP_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 65536, TMP_EINVAL,
               "%s: heads (%d) must be a multiple of kv_heads (%d), at most 65536", what, a->heads, a->kv_heads);
@@ -725,7 +725,7 @@ static int window_check(const tmp_window_attention_args *a, const char *what, bo
 static int window_params(const tmp_window_attention_args *a, const char *what, bool grad, WindowParams *p) {
   memset(p, 0, sizeof(*p));
   const int b = a->type == TMP_F32 ? 4 : 2;
-  p->s.offsets = a->offsets; p->s.n_series = a->offsets ? a->n_series : 1; p->s.n = (int32_t)a->n;
+  p->s.offsets = a->offsets; p->s.n_series = a->n_series; p->s.n = (int32_t)a->n;
   TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p->q);
   TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p->k);
   TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p->v);

@@ -76,3 +76,25 @@ def test_more_than_a_launch_holds_is_refused():
     a = _args(_lib.WindowCacheWriteArgs, n=100, n_series=600_000, offsets=4096, n_slots=600_000, type=0, kv_heads=1, dim_k=16,
               dim_v=16, window=1000, sinks=0, k=rows, v=rows, k_cache=cache, v_cache=cache, length=4096)
     assert h.tmp_window_cache_write(C.byref(a), None) == -4 and b"series x rows" in h.tmp_last_error()
+
+
+def test_numbers_of_series():
+    """Without offsets there is one series (none, or two, would be states that are not there); with them any number whose
+    arithmetic fits 32 bits."""
+    import ctypes as C
+    from tempo_amd import _lib
+    h = _lib.lib()
+    rows, cache = _lib.RowsRef(4096, 64, 16), _lib.CacheRef(4096, 640, 64, 16)
+    common = dict(n=0, type=0, dim_k=16, dim_v=16, q=rows, k=rows, v=rows)
+    calls = {
+        "tmp_window_attention": (_args(_lib.WindowAttentionArgs, **common, heads=2, kv_heads=2, window=5, scale=1.0, out=rows), (None,)),
+        "tmp_decay_attention": (_args(_lib.DecayAttentionArgs, **common, heads=2, scale=1.0, log_decay=4096, out=rows, state_out=4096),
+                                (None, 0, None)),
+        "tmp_window_cache_write": (_args(_lib.WindowCacheWriteArgs, n=0, type=0, dim_k=16, dim_v=16, kv_heads=2, window=5, n_slots=9,
+                                         k=rows, v=rows, k_cache=cache, v_cache=cache, length=4096), (None,)),
+    }
+    for name, (a, rest) in calls.items():
+        for offsets, n_series in ((None, 0), (None, 2), (4096, -1), (4096, 2 ** 31 - 65536), (4096, 2 ** 31 - 1)):
+            a.offsets, a.n_series = offsets, n_series
+            assert getattr(h, name)(C.byref(a), *rest) == -1, (name, offsets, n_series)
+            assert b"series" in h.tmp_last_error()
