@@ -549,7 +549,10 @@ static int decay_empty(const DecayParams &p, int64_t n_series, int64_t per_serie
 using namespace tmp;
 
 extern "C" size_t tmp_decay_attention_workspace_bytes(const tmp_decay_attention_args *a) {
-  if (!a || a->heads < 1 || a->dim_k < 1 || a->dim_v < 1) return 0;
+  // (what the call itself refuses needs none: no more is taken for it than for a call that runs)
+  if (!a || a->n < 0 || a->n >= (1ll << 31) - 65536 || a->heads < 1 || a->heads > 65536 || a->dim_k < 1 || a->dim_v < 1 ||
+      a->dim_k > TMP_MAX_HEAD_DIM || a->dim_v > TMP_MAX_HEAD_DIM)
+    return 0;
   Workspace ws(nullptr, 0);
   DecayPlan d;
   decay_plan(a, a->dout.p || a->n <= 0 ? 3 : 1, ws, &d);  // (without rows there may be no pointers)

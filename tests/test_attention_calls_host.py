@@ -98,3 +98,12 @@ def test_numbers_of_series():
             a.offsets, a.n_series = offsets, n_series
             assert getattr(h, name)(C.byref(a), *rest) == -1, (name, offsets, n_series)
             assert b"series" in h.tmp_last_error()
+
+
+def test_no_workspace_for_what_is_refused():
+    import ctypes as C
+    from tempo_amd import _lib
+    h = _lib.lib()
+    for change in (dict(dim_k=2 ** 20), dict(dim_v=129), dict(heads=65537), dict(n=2 ** 31 - 65536), dict(n=-1)):
+        a = _args(_lib.DecayAttentionArgs, **{**dict(n=10 ** 6, n_series=1, heads=8, dim_k=64, dim_v=64), **change})
+        assert h.tmp_decay_attention_workspace_bytes(C.byref(a)) == 0, change
