@@ -27,6 +27,7 @@ from ._lib import (CacheRef, DecayAttentionArgs, DecayAttentionStepArgs, RowsRef
                    WindowAttentionStepArgs, WindowCacheWriteArgs, check, lib)
 
 _TYPES = {torch.bfloat16: 0, torch.float32: 1}
+_MOST = 2 ** 31 - 65536  # series, slots: the library is told their number in 32 bits
 
 
 def _on_device(t, name, device=None):
@@ -43,7 +44,7 @@ def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
     if isinstance(t, torch.Tensor) and t.dim() == 3 and t.is_cuda and t.dtype in _TYPES:
         # the usual case, asked for at once: small calls are bound by their host part
         (rows, h, d), (row, _, last) = t.shape, t.stride()
-        if last == 1 and h and d and (rows <= 1 or d <= row < 2 ** 22):
+        if last == 1 and 0 < h <= 65536 and 0 < d <= 128 and (rows <= 1 or d <= row < 2 ** 22):
             if like is None:
                 return t
             if rows == n and heads in (None, h) and dim in (None, d) and t.dtype is like.dtype and t.device == like.device:
@@ -60,6 +61,8 @@ def _rows_check(t, name, like=None, n=None, heads=None, dim=None):
             raise ValueError(f"{name} has {have} {what}, expected {want}")
     if t.shape[1] < 1 or t.shape[2] < 1:
         raise ValueError(f"{name} needs at least one head and one element")
+    if t.shape[1] > 65536 or t.shape[2] > 128:  # (asked here too: the library is told them in 32 bits)
+        raise NotImplementedError(f"{name} has {t.shape[1]} heads of {t.shape[2]} elements, limited to 65536 of 128")
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name} must be contiguous in its innermost dimension")
     return t if t.shape[0] <= 1 or t.shape[2] <= t.stride(0) < 2 ** 22 else t.contiguous()
@@ -82,6 +85,8 @@ def _offsets_check(offsets, device):
     _on_device(offsets, "offsets", device)
     if offsets.dtype != torch.int64 or offsets.dim() != 1 or not offsets.is_contiguous() or offsets.numel() < 1:
         raise ValueError("offsets must be a contiguous int64 vector of at least one element")
+    if offsets.numel() > _MOST:
+        raise ValueError(f"offsets of {offsets.numel() - 1} series, at most {_MOST - 1}")
     return offsets.numel() - 1
 
 
@@ -125,10 +130,11 @@ def _changed(*tensors):
     torch.autograd.graph.increment_version(tensors)
 
 
-def _int_arg(value, name, low):
+def _int_arg(value, name, low, most):
+    """An integer >= low; what is above `most` is handed on as that."""
     if isinstance(value, bool) or int(value) != value or value < low:
         raise ValueError(f"{name} must be an integer >= {low}")
-    return int(value)
+    return min(int(value), most)
 
 
 def series_offsets(key, n_keys):
@@ -237,6 +243,8 @@ def decay_attention(q, k, v, log_decay, offsets=None, scale=None, state=None, re
 
 
 def _slots_check(slots, n, n_slots, device):
+    if n_slots >= _MOST:
+        raise ValueError(f"{n_slots} slots, at most {_MOST - 1}")
     if slots is None:
         if n != n_slots:
             raise ValueError(f"{n} rows for {n_slots} slots: slots must say which")
@@ -289,8 +297,8 @@ def _window_args(q, k, v, window, sinks, offsets, scale):
         raise ValueError(f"{heads} query heads cannot share {kv} key/value heads")
     n_series = _offsets_check(offsets, q.device)
     a = WindowAttentionArgs(n=n, n_series=n_series, offsets=_p(offsets), type=_TYPES[q.dtype], heads=heads, kv_heads=kv,
-                            dim_k=dk, dim_v=v.shape[2], window=min(_int_arg(window, "window", 1), 2 ** 62),
-                            sinks=_int_arg(sinks, "sinks", 0), scale=_scale(scale, dk), q=_ref(q), k=_ref(k), v=_ref(v))
+                            dim_k=dk, dim_v=v.shape[2], window=_int_arg(window, "window", 1, 2 ** 62),
+                            sinks=_int_arg(sinks, "sinks", 0, 2 ** 31 - 1), scale=_scale(scale, dk), q=_ref(q), k=_ref(k), v=_ref(v))
     a.held = (q, k, v)
     return a
 
@@ -368,8 +376,10 @@ def _caches_check(k_cache, v_cache, length, sinks, like, kv_heads, dk, dv):
             raise ValueError(f"{name} must not repeat its rows (expanded tensor)")
     if k_cache.shape[:2] != v_cache.shape[:2]:
         raise ValueError("k_cache and v_cache must have the same slots and rows")
-    sinks = _int_arg(sinks, "sinks", 0)
+    sinks = _int_arg(sinks, "sinks", 0, 2 ** 31 - 1)
     window = k_cache.shape[1] - sinks
+    if window >= 2 ** 30:
+        raise ValueError(f"a cache of {k_cache.shape[1]} rows: its window must be below 2^30")
     if window < 1:
         raise ValueError(f"a cache of {k_cache.shape[1]} rows has no window behind {sinks} sinks")
     _plain_check(length, "length", torch.int64, (k_cache.shape[0],), like.device)

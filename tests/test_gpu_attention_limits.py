@@ -326,3 +326,36 @@ def test_more_series_than_a_launch_has_blocks():
     assert torch.equal(last[full], ops.decay_attention(q, k, v, ld, offsets=small, state=state[full].contiguous(), return_state=True)[1])
     _, last = ops.decay_attention(q, k, v, ld, offsets=off, return_state=True)
     assert not bool(last[empty].any())
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Numbers that the library is told in 32 bits do not come out as others."""
+    from tempo_amd import ops
+    a = torch.zeros(3, 1, 8, device="cuda")
+    ld = torch.zeros(1, device="cuda")
+    for sinks in (2 ** 32, 2 ** 32 + 2, 2 ** 70):
+        with pytest.raises(NotImplementedError, match="sinks"):
+            ops.window_attention(a, a, a, 5, sinks=sinks)
+    wide = torch.zeros(3, 1, 1, device="cuda").expand(3, 2 ** 32 + 1, 1)
+    for call in (lambda: ops.window_attention(wide, wide, wide, 5), lambda: ops.window_attention(wide, a[..., :1], a[..., :1], 5),
+                 lambda: ops.decay_attention(wide, wide, wide, ld)):
+        with pytest.raises(NotImplementedError, match="heads"):
+            call()
+    long = torch.empty(2 ** 32 + 8, device="cuda", dtype=torch.bfloat16).reshape(1, 1, -1)
+    with pytest.raises(NotImplementedError, match="elements"):
+        ops.window_attention(long, long, long, 5)
+    cache = long.reshape(1, -1, 1, 1)  # 2^32 + 8 rows
+    b = torch.zeros(1, 1, 1, device="cuda", dtype=torch.bfloat16)
+    length = torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="window"):
+        ops.window_attention_step(b, b, b, cache, cache, length)
+    with pytest.raises(ValueError, match="window"):
+        ops.window_cache_write(b, b, cache, cache, length)
+    del cache, long
+    some = torch.zeros(1, dtype=torch.int32, device="cuda")
+    one = torch.zeros(1, 1, 1, device="cuda")
+    state = torch.empty(2 ** 31, 1, 1, 1, device="cuda")
+    with pytest.raises(ValueError, match="slots"):
+        ops.decay_attention_step(one, one, one, ld, state, slots=some)
+    with pytest.raises(ValueError, match="series"):
+        ops.window_attention(one, one, one, 5, offsets=torch.empty(2 ** 31, dtype=torch.int64, device="cuda"))
