@@ -141,9 +141,10 @@ def series_offsets(key, n_keys):
     """Where each series of a table in (key, ts) order starts: int64 [n_keys + 1] on the device, from the
     key column (int32, ids in [0, n_keys))."""
     from . import ops
-    counts = ops.key_counts(key, n_keys)
-    offsets = torch.zeros(n_keys + 1, dtype=torch.int64, device=counts.device)
-    torch.cumsum(counts.to(torch.int64), 0, out=offsets[1:])
+    with _current(_on_device(key, "key").device):
+        counts = ops.key_counts(key, n_keys)
+        offsets = torch.zeros(n_keys + 1, dtype=torch.int64, device=counts.device)
+        torch.cumsum(counts, 0, out=offsets[1:])
     return offsets
 
 

@@ -41,6 +41,32 @@ def test_forward_mode_is_refused():
                 call()
 
 
+def test_series_offsets_runs_on_the_device_of_its_keys(monkeypatch):
+    """key_counts launches on the current device's stream: the keys' device is made the current one around it."""
+    import contextlib
+    from tempo_amd import attention, ops
+    entered = []
+
+    @contextlib.contextmanager
+    def current(device):
+        entered.append(device)
+        yield
+        entered.append(None)
+
+    def key_counts(key, n_keys):
+        assert entered == [key.device]
+        return torch.tensor([2, 0, 3])
+
+    monkeypatch.setattr(attention, "_current", current)
+    monkeypatch.setattr(attention, "_on_device", lambda t, *_: t)
+    monkeypatch.setattr(ops, "key_counts", key_counts)
+    assert ops.series_offsets(torch.zeros(5, dtype=torch.int32), 3).tolist() == [0, 2, 2, 5]
+    assert len(entered) == 2
+    monkeypatch.undo()
+    with pytest.raises(TypeError, match="no CPU path"):
+        ops.series_offsets(torch.zeros(5, dtype=torch.int32), 3)
+
+
 def _args(cls, **kw):
     a = cls()
     for name, value in kw.items():
