@@ -356,6 +356,10 @@ __global__ __launch_bounds__(kBlock, TEMPO_RM_OCC) void route_move_kernel(int64_
 // the flush skips empty counters.
 constexpr int kCountLds = 12288;
 
+__global__ __launch_bounds__(kBlock) void clear_counts_kernel(int64_t *counts, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock) counts[i] = 0;
+}
+
 __global__ __launch_bounds__(kBlock) void key_counts_kernel(const int32_t *__restrict__ key, int64_t n_samples,
                                                             int64_t stride, uint32_t n_keys,
                                                             unsigned long long *counts) {
@@ -516,7 +520,9 @@ extern "C" int tmp_key_counts(const tmp_key_counts_args *a, void *, size_t, void
   TMP_REQUIRE(a->n_keys >= 1 && a->out_counts, TMP_EINVAL, "tmp_key_counts: n_keys >= 1 and out_counts needed");
   TMP_REQUIRE(a->stride >= 1, TMP_EINVAL, "tmp_key_counts: stride must be >= 1");
   hipStream_t st = (hipStream_t)stream;
-  TMP_CHECK_HIP(hipMemsetAsync(a->out_counts, 0, sizeof(int64_t) * (size_t)a->n_keys, st));
+  // (a kernel rather than a memset: the call may be captured, and memset nodes do not clear on every replay)
+  TMP_LAUNCH(clear_counts_kernel, dim3(grid_for(a->n_keys, kBlock, 1024)), dim3(kBlock), st, a->out_counts, (int64_t)a->n_keys);
+  TMP_CHECK_HIP(hipGetLastError());
   if (a->n == 0) return TMP_OK;
   TMP_REQUIRE(a->key, TMP_EINVAL, "tmp_key_counts: null key column");
   const int64_t n_samples = (a->n + a->stride - 1) / a->stride;

@@ -359,3 +359,41 @@ def test_sizes_beyond_32_bits_are_refused():
         ops.decay_attention_step(one, one, one, ld, state, slots=some)
     with pytest.raises(ValueError, match="series"):
         ops.window_attention(one, one, one, 5, offsets=torch.empty(2 ** 31, dtype=torch.int64, device="cuda"))
+
+
+def test_a_table_captured_from_its_keys_on():
+    """Offsets from the key column and both operators in one graph, replayed over other tables of the same size with eager
+    work in between."""
+    from tempo_amd import ops
+    n, n_keys, h, d = 900, 12, 2, 32
+    g = torch.Generator(device="cuda").manual_seed(29)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda") for _ in range(3))
+    ld = torch.tensor([-0.1, -0.01], device="cuda")
+    key = torch.zeros(n, dtype=torch.int32, device="cuda")
+    tables = [torch.sort(torch.randint(0, n_keys, (n,), generator=g, device="cuda", dtype=torch.int32)).values for _ in range(4)]
+
+    def step():
+        off = ops.series_offsets(key, n_keys)
+        return off, ops.window_attention(q, k, v, 20, sinks=1, offsets=off), ops.decay_attention(q, k, v, ld, offsets=off)
+
+    want = []
+    for t in tables:
+        key.copy_(t)
+        want.append([x.clone() for x in step()])
+        assert want[-1][0].tolist() == [0] + torch.bincount(t.long(), minlength=n_keys).cumsum(0).tolist()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in (0, 1, 2, 3, 1, 0):
+        key.copy_(tables[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want[i]):
+            assert torch.equal(a, b)
+        ops.key_counts(tables[2], n_keys)
+        torch.randn(1000, device="cuda").sum().item()
