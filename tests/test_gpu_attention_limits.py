@@ -397,3 +397,27 @@ def test_a_table_captured_from_its_keys_on():
             assert torch.equal(a, b)
         ops.key_counts(tables[2], n_keys)
         torch.randn(1000, device="cuda").sum().item()
+
+
+def test_window_attention_of_the_largest_table():
+    """2^31 - 65537 rows in series of a million, a few rows of window and two that stay visible: the last rows' results are
+    those of a short series that holds what they see."""
+    from tempo_amd import ops
+    n, m, window, sinks, look = 2 ** 31 - 65537, 1_000_000, 5, 2, 3_000
+    period = 6_400
+    g = torch.Generator().manual_seed(31)
+    small = [torch.randn(period, 1, 1, generator=g).to(torch.bfloat16) for _ in range(4)]
+    q, k, v, do = (x.cuda().repeat(-(-n // period), 1, 1)[:n] for x in small)
+    off = torch.cat([torch.arange(0, n, m, device="cuda"), torch.tensor([n], device="cuda")])
+    start = (n - 1) // m * m
+    junk = [torch.full((n, 1, 1), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    del junk
+    out, lse = ops.window_attention(q, k, v, window, sinks=sinks, offsets=off, return_lse=True)
+    grads = ops.window_attention_grad(do, q, k, v, out, lse, window, sinks=sinks, offsets=off)
+    rows = torch.cat([torch.arange(start, start + sinks), torch.arange(n - look, n)]).cuda()
+    want = ref.window_reference(*(x[rows].cpu() for x in (q, k, v, do)), [0, len(rows)], window, sinks, 1.0)
+    whole = slice(sinks + window, None)  # (before them the short series lacks rows; its first rows' dk, dv too)
+    for name, x in (("out", out), ("lse", lse), *zip(("dq", "dk", "dv"), grads)):
+        ref.check(name, x[rows][whole], want[name][0][whole], want[name][1][whole])
+    for x in (out, *grads):
+        assert all(bool(part.isfinite().all()) for part in x.split(1 << 28))
