@@ -15,7 +15,9 @@
 
 namespace tmp {
 
-// The slot of row b, -1 if it has none of its own.  All threads of the wave call this together.
+// The slot of row b, -1 if it has none of its own.  All threads of the wave call this together.  Every block looks through
+// the slots of the rows before its own: nothing to speak of up to 512 rows, but a decay step of 4096 rows x 16 x 64 takes
+// 678 us with slots and 378 without, of the most rows (65536 x 8 x 32) 31 and 1.9 ms.
 __device__ inline int slot_of(const int32_t *slots, int b, int n_slots) {
   if (!slots) return b;
   const int s = slots[b];

@@ -99,7 +99,8 @@ template <int NT> __device__ inline void state_store(const f32x16 (&st)[NT], flo
 }
 
 // X <- X + K^T diag(w) V for sixteen rows.  The weighted values do not fit bfloat16; they enter as the sum
-// of two such numbers (2^-18 of a term), three where the state itself is returned (2^-27).
+// of two such numbers, which leave 2^-17 of a term at most, three where the state itself is returned, which leave nothing
+// (all 24 bits of it).
 template <int D, bool EXACT> __device__ inline void state_add(f32x16 (&st)[D / 32], const __bf16 *kt, int k0, const float *w, bf16x8 v, int) {
   bf16x8 hi, lo;
   f32x8 x;
@@ -140,9 +141,13 @@ constexpr int da_waves(int dk, int dv) { return dv < dk ? 1 : 2; }
 //
 // A wave owns 32 columns of the values and that strip of the state, in registers; the queries', keys' and
 // values' tiles (da_piece rows) are shared, the next ones on their way meanwhile.  Rows are worked on in parts of
-// SUB, whose decays are the same for every part but a series' last one.  Memory bounds it once there are rows enough:
-// 131072 x 16 x 128 bf16 514 us, 4.2 TB/s (states alone 224 us, 4.8 TB/s); 50000 x 16 x 64 bf16, the backward pass's
-// three 312 us, 3.9 TB/s; float by its matrix instructions (30011 x 8 x 40/72: 150 us).
+// SUB, whose decays are the same for every part but a series' last one.  With bfloat16 rows the decayed scores and the
+// state itself enter the products that make a row's result as one bfloat16 number each, off by 2^-8 of a term at most (the
+// state that is carried, handed on and returned stays in 32 bits): errors of 2.3e-3 against 64 bits, of which rounding the
+// result is 1.66e-3; a second product for each would add nearly a third to the walk's matrix instructions.
+// Memory bounds it once there are rows enough: 131072 x 16 x 128 bf16 506 us, 4.2 TB/s (states alone 231 us, 4.6 TB/s);
+// 50000 x 16 x 64 bf16, the backward pass's three 313 us, 3.9 TB/s; float by its matrix instructions (30011 x 8 x 40/72:
+// 150 us).
 template <typename T, int DK, int DV, bool VEC, bool OUT, bool EXACT>
 __global__ __launch_bounds__(DV * 2, da_waves(DK, DV)) void decay_walk_kernel(DecayWalks w) {
   const DecayParams &p = w.p[blockIdx.y];
@@ -424,8 +429,9 @@ __global__ __launch_bounds__(256) void decay_empty_kernel(DecayParams p, int64_t
 // ---- host ----------------------------------------------------------------------------------------
 
 // Sections of whole pieces, as few as give the 1024 SIMDs the two waves each that they hold (a block has one for 32 of
-// dv): every one more adds a state to be written, strung together and read.  131072 x 16 x 128 bf16: 512 blocks 913 us,
-// 1024 955 us, 2048 1017 us; 50000 x 16 x 64: a walk takes 113 us with 1024 or 2048 blocks, 120 us with 512.
+// dv): every one more adds a state to be written, strung together and read.  131072 x 16 x 128 bf16: 256 blocks 1057 us,
+// 512 829 us, 1024 860 us, 2048 921 us; training of 50000 x 16 x 64: 512 blocks 544 us, 1024 539 us, 2048 609 us; 30011 x
+// 8 x 40/72 float: 256 blocks 253 us, 512 219 us, 1024 227 us.
 static int decay_section(int64_t n, int heads, int dim) {
   const int dv = padded_dim(dim);  // the larger of the two sizes: either is the values' in some walk
   const int blocks = 2048 / (dv / 32);

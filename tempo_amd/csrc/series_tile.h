@@ -58,7 +58,7 @@ __device__ inline f32x16 zero16() {
 }
 
 // Registers 8 * b .. 8 * b + 7 of a result as the operand of a product's step b.  To bf16: rounded to
-// nearest even, half a step of 2^-8 relative at most; the sums of the product stay in 32 bits.
+// nearest even, off by 2^-8 of the value at most; the sums of the product stay in 32 bits.
 template <typename T> __device__ inline Frag<T> operand(const f32x16 &c, int b);
 template <> __device__ inline bf16x8 operand<__bf16>(const f32x16 &c, int b) {
   bf16x8 f;

@@ -224,10 +224,12 @@ __device__ inline void store_own(const f32x16 (&acc)[NT], float by, const Rows &
   }
 }
 
-// Bound by the matrix cores and the vector unit together: an element of a part costs 4 D operations and some ten vector
-// instructions (scale, maximum, exponential, sum, rounding), which take as long as the products at D = 64 and half as
-// long at 128.  131072 x 16 x 128, window 600: 1.10 ms, 577 TFLOP/s of visible pairs; 32768 x 16 x 64, window 1000:
-// 216 us, 537 TFLOP/s (library products reach 1134).  Waves a SIMD: as many as fit the registers without spilling.
+// An element of a part costs 4 D operations and some ten vector instructions (scale, maximum, exponential, sum, rounding),
+// which take as long as the products at D = 64 and half as long at 128.  131072 x 16 x 128, window 600: 1.09 ms, 583
+// TFLOP/s of visible pairs; 32768 x 16 x 64, window 1000: 216 us, 537 TFLOP/s (library products reach 1134).  At 64 vector
+// issue bounds it (0.64 of the cycles); at 128 nothing is full (matrix cores 0.31, vector issue 0.42, LDS 0.26): the chain
+// product, maximum, exponential, product of 32 rows is waited for by two waves a SIMD.  Waves a SIMD: as many as fit the
+// registers but for a few values (spilled: bf16 of 128 two, twelve for rows of odd sizes; float of 128 25 to 28).
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) == 128 ? 3 : 2) void window_forward_kernel(WindowParams p, int tiles) {
   // float: matrix instructions are a sixteenth as fast, and parts that a wave does not see are left out one by one
@@ -395,7 +397,8 @@ __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) == 128 ? 3 : 2) void wind
 }
 
 // dq, and do.o for the kernel that follows.  Scores are computed again: 6 D operations for each element and no running
-// maximum, and 2 D more for the rest of dS.  32768 x 16 x 64, window 1000: 294 us, 790 TFLOP/s with those.
+// maximum, and 2 D more for the rest of dS.  32768 x 16 x 64, window 1000: 298 us, 780 TFLOP/s with those.  bf16 of 128
+// spills 15 registers (25 for rows of odd sizes).
 template <typename T, int D, bool VEC>
 __global__ __launch_bounds__(WA_THREADS, D * sizeof(T) >= 512 ? 1 : 2) void window_dq_kernel(WindowParams p, int tiles) {
   const int item = item_of_block(tiles * p.heads);
@@ -498,7 +501,8 @@ constexpr int wa_waves(int bytes, int d) { return d * bytes < 256 || (d * bytes 
 // dk and dv: a block owns key rows and streams the query rows that see them, head after head of the
 // group that shares them.  SINK: the rows that stay visible, against the query rows of one section
 // that lie beyond what the other form adds; leaves its sums as a part for sink_sum_kernel.
-// 32768 x 16 x 64 sharing 4, window 1000: 354 us, 656 TFLOP/s (8 D operations an element); its four sinks 41 us.
+// 32768 x 16 x 64 sharing 4, window 1000: 406 us, 715 TFLOP/s (10 D operations an element); its four sinks 43 us.  Heads
+// of 128, window 600: 848 us, one wave a SIMD.
 template <typename T, int D, bool VEC, bool SINK>
 __global__ __launch_bounds__(WA_THREADS, wa_waves(sizeof(T), D)) void window_dkdv_kernel(WindowParams p, int tiles) {
   constexpr bool TIGHT = wa_tight(sizeof(T), D);
