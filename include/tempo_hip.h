@@ -748,7 +748,7 @@ int tmp_arrow_import(const struct ArrowArray *array, const struct ArrowSchema *s
  * series after the other, as tmp_sort_order leaves them; offsets is a DEVICE array of n_series + 1
  * ascending row numbers, series s being rows [offsets[s], offsets[s + 1]).  Rows before the first or
  * behind the last offset belong to no series: their results are zeros and nothing reads them.  NULL
- * offsets: one series of all rows, n_series 1.
+ * offsets: one series of all rows (n_series is 1, or was left 0; tmp_window_cache_write writes n_series slots).
  *
  * Row arrays: element d of head h of row r at p[r * row_stride + h * head_stride + d] (strides in
  * elements), of type TMP_BF16 or TMP_F32; row_stride (the cache's too) is at least the head size and

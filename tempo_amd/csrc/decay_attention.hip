@@ -531,7 +531,7 @@ static void decay_run(const DecayWalks &w, int walks, int type, hipStream_t st) 
 static DecayParams decay_params(const tmp_decay_attention_args *a, const DecayPlan &d, int walk) {
   DecayParams p;
   memset(&p, 0, sizeof(p));
-  p.s.offsets = a->offsets; p.s.n_series = a->n_series; p.s.n = (int32_t)a->n;
+  p.s.offsets = a->offsets; p.s.n_series = a->offsets ? a->n_series : 1; p.s.n = (int32_t)a->n;
   p.log_decay = a->log_decay;
   p.carry = d.carry + walk * d.per_walk; p.link = d.link + walk * (d.sections + 1); p.section = d.section; p.sections = d.sections;
   // Few rows: one launch, whose blocks walk the rows of their first series that lie before them once more, costs less than

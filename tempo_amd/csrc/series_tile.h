@@ -460,13 +460,14 @@ __device__ inline int item_of_block(int total) {
 inline int grid_of_items(int64_t total) { return (int)((total + 7) / 8 * 8); }
 
 // ---- host side -------------------------------------------------------------------------------
-// Without offsets there is one series; numbers of series are compared with 32-bit arithmetic beside that of rows.
+// Without offsets there is one series, also where n_series was left zero; numbers of series are compared with 32-bit
+// arithmetic beside that of rows.
 inline bool series_ok(const int64_t *offsets, int32_t n_series) {
-  return offsets ? n_series >= 0 && n_series < kNoSeries : n_series == 1;
+  return n_series >= 0 && n_series < (offsets ? kNoSeries : 2);
 }
 #define TMP_SERIES(what, a)                                                                                     \
   TMP_REQUIRE(series_ok((a)->offsets, (a)->n_series), TMP_EINVAL,                                               \
-              "%s: bad series: their number must be in [0, 2^31 - 65536), 1 without offsets", what)
+              "%s: bad series: their number must be in [0, 2^31 - 65536), at most 1 without offsets", what)
 // Rows of `n`, dim elements each; false: strides that the kernels do not take.
 inline bool rows_of(const tmp_rows &r, int64_t n, int dim, int bytes, Rows *o) {
   const int64_t per = 16 / bytes;

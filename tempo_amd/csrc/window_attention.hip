@@ -729,7 +729,7 @@ static int window_check(const tmp_window_attention_args *a, const char *what, bo
 static int window_params(const tmp_window_attention_args *a, const char *what, bool grad, WindowParams *p) {
   memset(p, 0, sizeof(*p));
   const int b = a->type == TMP_F32 ? 4 : 2;
-  p->s.offsets = a->offsets; p->s.n_series = a->n_series; p->s.n = (int32_t)a->n;
+  p->s.offsets = a->offsets; p->s.n_series = a->offsets ? a->n_series : 1; p->s.n = (int32_t)a->n;
   TMP_ROWS(what, a->q, a->n, a->dim_k, b, &p->q);
   TMP_ROWS(what, a->k, a->n, a->dim_k, b, &p->k);
   TMP_ROWS(what, a->v, a->n, a->dim_v, b, &p->v);

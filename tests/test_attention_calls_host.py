@@ -105,8 +105,7 @@ def test_more_than_a_launch_holds_is_refused():
 
 
 def test_numbers_of_series():
-    """Without offsets there is one series (none, or two, would be states that are not there); with them any number whose
-    arithmetic fits 32 bits."""
+    """Without offsets there is one series, with them any number whose arithmetic fits 32 bits."""
     import ctypes as C
     from tempo_amd import _lib
     h = _lib.lib()
@@ -120,10 +119,14 @@ def test_numbers_of_series():
                                          k=rows, v=rows, k_cache=cache, v_cache=cache, length=4096), (None,)),
     }
     for name, (a, rest) in calls.items():
-        for offsets, n_series in ((None, 0), (None, 2), (4096, -1), (4096, 2 ** 31 - 65536), (4096, 2 ** 31 - 1)):
+        for offsets, n_series in ((None, -1), (None, 2), (4096, -1), (4096, 2 ** 31 - 65536), (4096, 2 ** 31 - 1)):
             a.offsets, a.n_series = offsets, n_series
             assert getattr(h, name)(C.byref(a), *rest) == -1, (name, offsets, n_series)
             assert b"series" in h.tmp_last_error()
+    a, rest = calls["tmp_window_attention"]
+    for offsets, n_series in ((None, 0), (None, 1), (4096, 0)):  # (no rows: nothing is launched)
+        a.offsets, a.n_series = offsets, n_series
+        assert h.tmp_window_attention(C.byref(a), *rest) == 0
 
 
 def test_no_workspace_for_what_is_refused():
