@@ -754,8 +754,8 @@ int tmp_arrow_import(const struct ArrowArray *array, const struct ArrowSchema *s
  * elements), of type TMP_BF16 or TMP_F32; row_stride (the cache's too) is at least the head size and
  * below 2^22, p a multiple of the type's size.  Outputs overlap neither an input nor each other.  Sums, softmax statistics
  * and states are 32-bit floats: scaled scores are to stay below 2^29 in magnitude, beyond which the weights of the window
- * form overflow.  A call has at most 2^24 - 8 heads x 128 rows (whole series), heads x rows (steps), series x 32 rows of a
- * cache (cache writes).
+ * form overflow.  A call has at most 2^24 - 8 heads x 128 rows (window, whole series), heads x rows (decay steps; window
+ * steps twice that), series x 32 rows of a cache (cache writes).
  * A value that is not finite makes the results that depend on it not finite (NaN or infinite), and
  * no other ones.  Calls enqueue work and return; none of them waits for the device.
  */

@@ -27,7 +27,7 @@ from ._lib import (CacheRef, DecayAttentionArgs, DecayAttentionStepArgs, RowsRef
                    WindowAttentionStepArgs, WindowCacheWriteArgs, check, lib)
 
 _TYPES = {torch.bfloat16: 0, torch.float32: 1}
-_MOST = 2 ** 31 - 65536  # series, slots: the library is told their number in 32 bits
+_MOST = 2 ** 31 - 65536  # series: the library is told their number in 32 bits, and compares with others beside it
 
 
 def _on_device(t, name, device=None):
@@ -244,8 +244,8 @@ def decay_attention(q, k, v, log_decay, offsets=None, scale=None, state=None, re
 
 
 def _slots_check(slots, n, n_slots, device):
-    if n_slots >= _MOST:
-        raise ValueError(f"{n_slots} slots, at most {_MOST - 1}")
+    if n_slots >= 2 ** 31:
+        raise ValueError(f"{n_slots} slots, at most {2 ** 31 - 1}: the library is told their number in 32 bits")
     if slots is None:
         if n != n_slots:
             raise ValueError(f"{n} rows for {n_slots} slots: slots must say which")

@@ -373,7 +373,6 @@ static int step_check_common(int64_t n, int32_t n_slots, const int32_t *slots, i
   TMP_REQUIRE(n_slots >= 0 && (slots || n <= n_slots), TMP_EINVAL, "%s: more rows than slots", what);
   TMP_REQUIRE(type == TMP_BF16 || type == TMP_F32, TMP_EUNSUPPORTED, "%s: type must be bfloat16 or float32", what);
   TMP_REQUIRE(heads > 0 && heads <= 65536, TMP_EINVAL, "%s: heads must be in [1, 65536]", what);
-  TMP_REQUIRE(n * heads <= kMostBlocks, TMP_EUNSUPPORTED, "%s: too many rows x heads, at most 2^24 - 8", what);
   TMP_REQUIRE(dk > 0 && dv > 0, TMP_EINVAL, "%s: head sizes must be positive", what);
   TMP_REQUIRE(dk <= TMP_MAX_HEAD_DIM && dv <= TMP_MAX_HEAD_DIM, TMP_EUNSUPPORTED, "%s: head sizes are limited to %d", what,
               TMP_MAX_HEAD_DIM);
@@ -383,6 +382,7 @@ static int step_check_common(int64_t n, int32_t n_slots, const int32_t *slots, i
 static int window_step_check(const tmp_window_attention_step_args *a, const char *what) {
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_TRY(step_check_common(a->n, a->n_slots, a->slots, a->type, a->heads, a->dim_k, a->dim_v, what));
+  TMP_REQUIRE(a->n * a->heads <= 2 * kMostBlocks, TMP_EUNSUPPORTED, "%s: too many rows x heads, at most 2^25 - 16", what);
   TMP_REQUIRE(a->kv_heads > 0 && a->heads % a->kv_heads == 0, TMP_EINVAL, "%s: heads must be a multiple of kv_heads", what);
   TMP_REQUIRE(a->window >= 1 && a->window < (1 << 30), TMP_EINVAL, "%s: window must be in [1, 2^30)", what);
   TMP_REQUIRE(a->sinks >= 0, TMP_EINVAL, "%s: sinks must be >= 0", what);
@@ -424,6 +424,7 @@ extern "C" int tmp_decay_attention_step(const tmp_decay_attention_step_args *a, 
   const char *what = "tmp_decay_attention_step";
   TMP_REQUIRE(a != nullptr, TMP_EINVAL, "%s: null args", what);
   TMP_TRY(step_check_common(a->n, a->n_slots, a->slots, a->type, a->heads, a->dim_k, a->dim_v, what));
+  TMP_REQUIRE(a->n * a->heads <= kMostBlocks, TMP_EUNSUPPORTED, "%s: too many rows x heads, at most 2^24 - 8", what);
   TMP_REQUIRE(a->scale > 0.f && a->scale < INFINITY, TMP_EINVAL, "%s: scale must be positive and finite", what);
   if (a->n == 0) return TMP_OK;
   TMP_REQUIRE(a->q.p && a->k.p && a->v.p && a->out.p && a->log_decay && a->state, TMP_EINVAL, "%s: null pointer", what);

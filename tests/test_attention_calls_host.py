@@ -90,7 +90,7 @@ def test_more_than_a_launch_holds_is_refused():
     assert h.tmp_window_attention_grad_workspace_bytes(C.byref(a)) == 0
     a.heads = a.kv_heads = 1  # the largest table of one head fits
     assert h.tmp_window_attention_grad_workspace_bytes(C.byref(a)) > 0
-    for n, heads in ((most // 8 + 1, 8), (1 << 24, 1), (2 ** 15, 512)):
+    for n, heads in ((most // 4 + 1, 8), (1 << 24, 2), (2 ** 16, 512)):
         a = _args(_lib.DecayAttentionStepArgs, n=n, n_slots=n, type=0, heads=heads, dim_k=16, dim_v=16, scale=1.0, log_decay=4096,
                   q=rows, k=rows, v=rows, out=rows, state=4096)
         assert h.tmp_decay_attention_step(C.byref(a), None) == -4 and b"rows x heads" in h.tmp_last_error()
@@ -99,6 +99,11 @@ def test_more_than_a_launch_holds_is_refused():
                   sinks=1, scale=1.0, q=rows, k=rows, v=rows, out=rows, k_cache=cache, v_cache=cache, length=4096)
         assert h.tmp_window_attention_step(C.byref(a), None, 0, None) == -4 and b"rows x heads" in h.tmp_last_error()
         assert h.tmp_window_attention_step_workspace_bytes(C.byref(a)) == 0
+    a.n = a.n_slots = most  # (blocks of 128 threads join the parts: twice as many rows x heads as above)
+    a.heads = a.kv_heads = 2
+    assert h.tmp_window_attention_step_workspace_bytes(C.byref(a)) > 0
+    a = _args(_lib.DecayAttentionStepArgs, n=most + 1, n_slots=most + 1, type=0, heads=1, dim_k=16, dim_v=16, scale=1.0)
+    assert h.tmp_decay_attention_step(C.byref(a), None) == -4 and b"rows x heads" in h.tmp_last_error()
     a = _args(_lib.WindowCacheWriteArgs, n=100, n_series=600_000, offsets=4096, n_slots=600_000, type=0, kv_heads=1, dim_k=16,
               dim_v=16, window=1000, sinks=0, k=rows, v=rows, k_cache=cache, v_cache=cache, length=4096)
     assert h.tmp_window_cache_write(C.byref(a), None) == -4 and b"series x rows" in h.tmp_last_error()

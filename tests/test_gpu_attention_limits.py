@@ -421,3 +421,42 @@ def test_window_attention_of_the_largest_table():
         ref.check(name, x[rows][whole], want[name][0][whole], want[name][1][whole])
     for x in (out, *grads):
         assert all(bool(part.isfinite().all()) for part in x.split(1 << 28))
+
+
+def test_steps_of_the_most_rows():
+    """Close to as many rows x heads as a step takes: every row is added and read."""
+    from tempo_amd import ops
+    n, h, d = 2 ** 20 - 1, 16, 4
+    g = torch.Generator(device="cuda").manual_seed(37)
+    q, k, v = (torch.randn(n, h, d, generator=g, device="cuda") for _ in range(3))
+    state = torch.randn(n, h, d, d, generator=g, device="cuda")
+    ld = torch.linspace(-0.5, -0.01, h, device="cuda")
+    s = state.double() * torch.exp(ld.double())[:, None, None] + k.double()[..., None] * v.double()[..., None, :]
+    size = state.double().abs() + k.double().abs()[..., None] * v.double().abs()[..., None, :]
+    out = ops.decay_attention_step(q, k, v, ld, state, scale=0.5)
+    # (a sum of two, its power off by three steps at most; then four terms, the scale and a rounding)
+    assert bool(((state - s).abs() <= 6 * ref.E32 * size).all())
+    want = (q.double()[..., None] * s).sum(2) * 0.5
+    assert bool(((out - want).abs() <= 14 * ref.E32 * (q.double().abs()[..., None] * size).sum(2) * 0.5).all())
+    del state, s, size, want, out
+    h, window = 32, 3
+    q = torch.randn(n, h, d, generator=g, device="cuda")
+    k, v = (torch.randn(n, 1, d, generator=g, device="cuda") for _ in range(2))
+    kc, vc = (torch.randn(n, window, 1, d, generator=g, device="cuda") for _ in range(2))
+    length = torch.arange(n, device="cuda") % 7
+    seen = (length + 1).clamp(max=window)
+    keys, vals = kc.clone(), vc.clone()
+    at = torch.arange(n, device="cuda")
+    keys[at, length % window], vals[at, length % window] = k, v
+    out = ops.window_attention_step(q, k, v, kc, vc, length, scale=0.5)
+    assert torch.equal(kc, keys) and torch.equal(vc, vals) and torch.equal(length, at % 7 + 1)
+    for a in range(0, n, 1 << 18):
+        b = slice(a, a + (1 << 18))
+        scores = (q[b].double()[:, :, None] * keys[b, None, :, 0].double()).sum(3) * 0.5
+        on = torch.arange(window, device="cuda") < seen[b, None, None]
+        p = torch.softmax(scores.masked_fill(~on, -float("inf")), 2)
+        want = (p[..., None] * vals[b, None, :, 0].double()).sum(2)
+        size = (p[..., None] * vals[b, None, :, 0].double().abs()).sum(2)
+        # weights: a score of four terms, its scale, the change of base and the exponential's two steps
+        rel = 16 * ref.E32 * (1 + scores.abs().amax(2, keepdim=True)) + 8 * ref.E32
+        assert bool(((out[b] - want).abs() <= 2 * rel * size + ref.E32 * want.abs()).all())
